@@ -67,7 +67,8 @@ MTN_API const char* mtn_version(void);
  * and the kernel-specific detail word; `clear` resets it.  Codes: 1 page id
  * outside the pool, 2 seq_len negative or beyond its pages, 3 slot outside
  * the pool, 4 a bounded wait ran out, 5 position beyond a sequence's pages,
- * 6 a decode plan made for another grid or not a plan. */
+ * 6 a decode plan made for another grid or not a plan, 7 a token id, index
+ * pointer or mask row of mtn_logits_rules out of range (detail: the row). */
 MTN_API int mtn_device_error(int device, int clear, int32_t* code, int32_t* detail);
 
 /* Self-test of the bounded device waits (failure detection without a GPU
@@ -115,7 +116,8 @@ MTN_API int64_t mtn_kv_page_offset(const mtn_kv_layout* pool, int32_t layer, int
 
 enum {
   MTN_DTYPE_BF16 = 0,
-  MTN_DTYPE_F32 = 1
+  MTN_DTYPE_F32 = 1,
+  MTN_DTYPE_E4M3 = 2 /* 8-bit floats with a scale per row: mtn_add_rms_norm's output, mtn_w4_matvec's input */
 };
 
 /* Attention flags. */
@@ -200,6 +202,52 @@ MTN_API int mtn_qkv_prologue(const mtn_kv_layout* pool, int32_t layer, const voi
                              int32_t q_gated, int32_t num_q_heads, const float* q_norm_w1, const float* k_norm_w1,
                              float eps, const float* inv_freq, int32_t rotary_dim, const int32_t* positions,
                              const int64_t* slots, int64_t n_tokens, float* q_out, void* stream);
+
+/* Residual addition + RMSNorm in one launch (qwen model.rs:98-108 and the
+ * residual sums of model.rs:348-365), for rows of `hidden` elements (up to
+ * 32768), row strides in elements:
+ *   sum = x + residual       rounded to res_dtype; sum may be residual itself
+ *   y   = sum / sqrt(mean(sum^2) + eps) * w1      (the sum as it is stored)
+ * residual / sum: both NULL for a plain norm of x.  w1: (1 + w) per element,
+ * or NULL for ones.  out: bf16 or f32 (scales NULL), or e4m3 with one f32
+ * scale per row, scale = max(max|y| / 448, 2^-100), out = e4m3(y / scale).
+ * Means and y are f32; a row that holds a NaN or an infinity comes out as
+ * the formula says, NaN scale included.  Besides sum == residual no output
+ * may overlap an input. */
+MTN_API int mtn_add_rms_norm(const void* x, int32_t x_dtype, int64_t x_stride, const void* residual,
+                             int64_t res_stride, void* sum, int64_t sum_stride, int32_t res_dtype, const float* w1,
+                             float eps, int64_t n_rows, int32_t hidden, void* out, int32_t out_dtype,
+                             int64_t out_stride, float* scales, void* stream);
+
+/* Matrix-vector products with 4-bit weights and group scales (MyLinear,
+ * qwen model.rs:110-130, for the few rows of a decode step):
+ *   out[m][j] = x_scales[m] * sum_i x[m][i] * q[j][i] * s[j][i / group]
+ * q: integers -8..7, s: bf16, group 32, 64 or 128; any n and any k up to
+ * 65536 (a last group may be partial).  Weights are kept in the library's own
+ * layout: `packed` of mtn_w4_packed_bytes and `scales` of mtn_w4_scales_bytes
+ * bytes, 16-byte aligned device memory, made by
+ *   mtn_w4_quantize  from bf16 / f32 weights [n][k]: per group
+ *                    s = bf16(max|w| / 7), q = round(w / s); a group of
+ *                    zeros has s = 0, one with a NaN or an infinity s = NaN;
+ *   mtn_w4_pack      from codes int8 [n][k] (clamped to -8..7) and bf16
+ *                    scales [n][ceil(k / group)], row strides in elements;
+ * mtn_w4_dequantize writes the values q * s row-major as f32 (exact) or bf16
+ * (for many rows: a prompt's product on the backend's BLAS).
+ * mtn_w4_matvec: x bf16, f32, or e4m3 with x_scales (what mtn_add_rms_norm
+ * writes; NULL for the other types), n_rows up to 65535; sums in f32, out
+ * bf16 or f32; out must not overlap x.  Every call reads the weights at least
+ * once per 16 rows. */
+MTN_API size_t mtn_w4_packed_bytes(int64_t n, int64_t k);
+MTN_API size_t mtn_w4_scales_bytes(int64_t n, int64_t k, int32_t group);
+MTN_API int mtn_w4_quantize(const void* weight, int32_t dtype, int64_t stride, int64_t n, int64_t k, int32_t group,
+                            void* packed, void* scales, void* stream);
+MTN_API int mtn_w4_pack(const int8_t* codes, int64_t code_stride, const void* code_scales, int64_t scale_stride,
+                        int64_t n, int64_t k, int32_t group, void* packed, void* scales, void* stream);
+MTN_API int mtn_w4_dequantize(const void* packed, const void* scales, int64_t n, int64_t k, int32_t group, void* out,
+                              int32_t dtype, int64_t stride, void* stream);
+MTN_API int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float* x_scales, int64_t n_rows,
+                          const void* packed, const void* scales, int64_t n, int64_t k, int32_t group, void* out,
+                          int32_t out_dtype, int64_t out_stride, void* stream);
 
 /* Gather sequences back into the reference's contiguous cache layout
  * KVCacheState::Attention [num_kv_heads][seq_len][head_dim] (bf16):
@@ -362,6 +410,55 @@ MTN_API int mtn_argmax_rows(const float* logits, int64_t n_rows, int64_t vocab, 
 MTN_API size_t mtn_sample_rows_workspace_bytes(int64_t n_rows, int64_t vocab);
 MTN_API int mtn_sample_rows(const float* logits, const float* temperatures, int64_t n_rows, int64_t vocab,
                             int32_t* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What the requests of a batch ask of their logits (no counterpart in the
+ * reference, whose sample_token takes the logits as they are).  Device
+ * arrays; each group is optional (NULL).
+ *   history: row r's tokens hist_tokens[hist_indptr[r] .. hist_indptr[r+1])
+ *     (n_hist in all), of which the first prompt_lens[r] are its prompt (NULL:
+ *     none) and the rest generated; repetition[r] > 0, presence[r] and
+ *     frequency[r] (NULL: 1, 0, 0) are the row's penalties;
+ *   biases: bias_values[i] for token bias_tokens[i], bias_indptr[r] <= i <
+ *     bias_indptr[r+1] (n_bias in all); a token listed twice in a row: its
+ *     last entry counts;
+ *   mask: bit v % 32 of word v / 32 allows token v; n_masks mask rows
+ *     mask_stride words apart, row r using mask row mask_rows[r] (-1: none;
+ *     NULL: mask row r).
+ * Token ids outside the vocabulary are skipped, a malformed index pointer
+ * counts as an empty row and a mask row out of range as none, each recorded
+ * as device error 7. */
+typedef struct {
+  const int32_t* hist_indptr;
+  const int32_t* hist_tokens;
+  int64_t n_hist;
+  const int32_t* prompt_lens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_indptr;
+  const int32_t* bias_tokens;
+  const float* bias_values;
+  int64_t n_bias;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int32_t n_masks;
+  const int32_t* mask_rows;
+} mtn_logits_rules;
+
+/* out[r][v] from logits row r (bf16 or f32, rows row_stride elements apart),
+ * in f32, one rounded operation after the other:
+ *   x = in the history ? (x > 0 ? x / repetition : x * repetition) : x
+ *   x = x - frequency * (times generated);  x = x - presence if generated
+ *   x = x + bias;  x = allowed ? x : -inf
+ * out may be logits (f32, equal strides).  tokens (or NULL): the processed
+ * row's first strict maximum, as mtn_argmax_rows gives it (a row whose mask
+ * leaves nothing gives 0).  workspace: for tokens only,
+ * mtn_process_logits_workspace_bytes(n_rows) bytes, 8-byte aligned, zeroed
+ * once before first use and left zeroed by every call, one stream at a time. */
+MTN_API size_t mtn_process_logits_workspace_bytes(int64_t n_rows);
+MTN_API int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, int64_t n_rows, int64_t vocab,
+                               const mtn_logits_rules* rules, float* out, int64_t out_stride, int32_t* tokens,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Host mirror: page allocator (kv_pool.rs:4-69) + refcount extension       */

@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libmitten_kv.so"
 
 MTN_OK, MTN_EINVAL, MTN_ENOMEM, MTN_ECUDA, MTN_ETIMEOUT, MTN_EDEVICE = range(6)
-MTN_DTYPE_BF16, MTN_DTYPE_F32 = 0, 1
+MTN_DTYPE_BF16, MTN_DTYPE_F32, MTN_DTYPE_E4M3 = range(3)
 MTN_ATTN_PHANTOM_ZERO_SLOT = 1
 MTN_ATTN_PREFILL_ONE_TILE = 2
 MTN_ATTN_SPLIT_BF16 = 4
@@ -72,6 +72,26 @@ class BatchView(C.Structure):
     ]
 
 
+class LogitsRules(C.Structure):
+    _fields_ = [
+        ("hist_indptr", C.c_void_p),
+        ("hist_tokens", C.c_void_p),
+        ("n_hist", C.c_int64),
+        ("prompt_lens", C.c_void_p),
+        ("repetition", C.c_void_p),
+        ("presence", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("bias_indptr", C.c_void_p),
+        ("bias_tokens", C.c_void_p),
+        ("bias_values", C.c_void_p),
+        ("n_bias", C.c_int64),
+        ("mask", C.c_void_p),
+        ("mask_stride", C.c_int64),
+        ("n_masks", C.c_int32),
+        ("mask_rows", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes).  Mirrors include/mitten_kv.h one to one; the
 # test suite checks that every declared symbol is exported and listed here.
 SIGNATURES: dict[str, tuple] = {
@@ -119,6 +139,19 @@ SIGNATURES: dict[str, tuple] = {
                                    C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
                                    C.c_float, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
                                    C.c_void_p]),
+    "mtn_add_rms_norm": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                   C.c_int32, C.c_void_p, C.c_float, C.c_int64, C.c_int32, C.c_void_p, C.c_int32,
+                                   C.c_int64, C.c_void_p, C.c_void_p]),
+    "mtn_w4_packed_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "mtn_w4_scales_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32]),
+    "mtn_w4_quantize": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p,
+                                  C.c_void_p, C.c_void_p]),
+    "mtn_w4_pack": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32,
+                              C.c_void_p, C.c_void_p, C.c_void_p]),
+    "mtn_w4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int32,
+                                    C.c_int64, C.c_void_p]),
+    "mtn_w4_matvec": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p]),
     "mtn_kv_pages_bytes": (C.c_size_t, [C.POINTER(KvLayout), C.c_int64]),
     "mtn_kv_pages_pack": (C.c_int, [C.POINTER(KvLayout), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "mtn_kv_pages_unpack": (C.c_int, [C.POINTER(KvLayout), C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
@@ -126,6 +159,9 @@ SIGNATURES: dict[str, tuple] = {
     "mtn_sample_rows_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64]),
     "mtn_sample_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t,
                                   C.c_void_p]),
+    "mtn_process_logits_workspace_bytes": (C.c_size_t, [C.c_int64]),
+    "mtn_process_logits": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.POINTER(LogitsRules),
+                                     C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     # host mirror: page pool
     "mtn_page_pool_create": (C.c_int, [C.c_int64, C.c_int32, C.POINTER(C.c_void_p)]),
     "mtn_page_pool_destroy": (None, [C.c_void_p]),

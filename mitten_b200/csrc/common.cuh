@@ -92,7 +92,8 @@ enum DevErr : int {
   kDevErrBadSlot = 3,       // slot outside the pool
   kDevErrTimeout = 4,       // bounded wait ran out
   kDevErrBadPosition = 5,   // position beyond a sequence's pages
-  kDevErrBadPlan = 6        // decode plan made for another grid (detail: its grid) or not a plan (-1)
+  kDevErrBadPlan = 6,       // decode plan made for another grid (detail: its grid) or not a plan (-1)
+  kDevErrBadLogitRule = 7   // logits rules: token id, index pointer or mask row out of range (detail: row)
 };
 
 // ---------------------------------------------------------------- device side

@@ -356,6 +356,110 @@ def sample_rows(logits: torch.Tensor, temperatures: torch.Tensor, out: torch.Ten
     return out
 
 
+class LogitsRules:
+    """What the rows of a batch ask of their logits (mtn_logits_rules): CUDA tensors on one device, each group
+    optional.
+
+      history  hist_indptr [rows + 1], hist_tokens: int32 CSR of every row's tokens, the first prompt_lens [rows]
+               of them its prompt (none without it), the rest generated; f32 [rows] each, or None:
+               repetition (> 0; divides positive and multiplies negative logits of every token in the history),
+               presence (subtracted once from generated tokens), frequency (subtracted per occurrence)
+      biases   bias_indptr [rows + 1], bias_tokens (int32), bias_values (f32): added; a token listed twice in a
+               row takes its last entry
+      mask     int32 [masks, >= ceil(vocab / 32)], bit v % 32 of word v / 32 allows token v; mask_rows int32
+               [rows] picks each row's mask (-1: none), by default mask row r
+
+    The object keeps the tensors; their contents may change between calls."""
+
+    def __init__(self, hist_indptr=None, hist_tokens=None, prompt_lens=None, repetition=None, presence=None,
+                 frequency=None, bias_indptr=None, bias_tokens=None, bias_values=None, mask=None, mask_rows=None):
+        if (hist_indptr is None) != (hist_tokens is None):
+            raise ValueError("hist_indptr and hist_tokens come together")
+        if hist_indptr is None and any(t is not None for t in (prompt_lens, repetition, presence, frequency)):
+            raise ValueError("penalties need a history")
+        if not (bias_indptr is None) == (bias_tokens is None) == (bias_values is None):
+            raise ValueError("bias_indptr, bias_tokens and bias_values come together")
+        if mask is None and mask_rows is not None:
+            raise ValueError("mask_rows without a mask")
+        if bias_tokens is not None and bias_tokens.numel() != bias_values.numel():
+            raise ValueError("one bias value per bias token")
+        self._keep = {k: t for k, t in locals().items() if k not in ("self", "__class__") and t is not None}
+        self.rows = None  # every row, where nothing is given per row
+        self.device = None
+        for name, t in self._keep.items():
+            want = torch.float32 if name in ("repetition", "presence", "frequency", "bias_values") else torch.int32
+            if t.dtype != want or (name != "mask" and (t.dim() != 1 or not t.is_contiguous())):
+                raise ValueError(f"{name} must be a contiguous 1-D {want} tensor, got {t.dim()}-D {t.dtype}")
+            if self.device not in (None, t.device):
+                raise ValueError("the rules' tensors lie on different devices")
+            self.device = t.device
+            if name.endswith(("tokens", "values")) or name == "mask":
+                continue
+            rows = t.numel() - (1 if name.endswith("indptr") else 0)
+            if rows < 0 or self.rows not in (None, rows):
+                raise ValueError(f"{name} has another number of rows")
+            self.rows = rows
+        if mask is not None and (mask.dim() != 2 or mask.stride(1) != 1 and mask.shape[1] > 1
+                                 or mask.stride(0) < mask.shape[1] and mask.shape[0] > 1):
+            raise ValueError("mask must be a [masks, words] int32 tensor of unit-stride rows")
+        self.mask_words = None if mask is None else mask.shape[1]
+        self.masks = None if mask is None else (mask.shape[0], mask_rows is None)
+        n = lambda t: 0 if t is None else t.numel()  # noqa: E731
+        self.struct = L.LogitsRules(
+            _ptr(hist_indptr), _ptr(hist_tokens), n(hist_tokens), _ptr(prompt_lens), _ptr(repetition), _ptr(presence),
+            _ptr(frequency), _ptr(bias_indptr), _ptr(bias_tokens), _ptr(bias_values), n(bias_tokens), _ptr(mask),
+            0 if mask is None else (mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]),
+            0 if mask is None else mask.shape[0], _ptr(mask_rows))
+        self._ref = C.byref(self.struct)
+
+
+def logits_workspace(n_rows: int, device) -> torch.Tensor:
+    """Zeroed workspace for process_logits' greedy tokens (left zeroed by every call; one stream at a time)."""
+    return torch.zeros(max(int(L.lib().mtn_process_logits_workspace_bytes(n_rows)), 16), dtype=torch.uint8,
+                       device=device)
+
+
+def process_logits(logits: torch.Tensor, rules: LogitsRules, out: torch.Tensor | None = None,
+                   tokens: torch.Tensor | None = None, greedy: bool = False, workspace: torch.Tensor | None = None,
+                   stream=None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Penalties, biases and masks on logits [rows, vocab] (bf16 or f32) before sampling: (out f32, tokens).
+
+    `out` may be the f32 logits themselves.  With `tokens` (int32 [rows]) or `greedy` the first strict maximum of
+    every processed row comes back too, as argmax_rows gives it; that needs `workspace` (logits_workspace; a fresh
+    one is made when none is given)."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (
+            logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be a [rows, vocab] f32 or bf16 tensor of unit-stride rows")
+    if logits.is_cuda and logits.device.index != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return process_logits(logits, rules, out, tokens, greedy, workspace, stream)
+    n, vocab = logits.shape
+    if rules.rows not in (None, n):
+        raise ValueError(f"rules for {rules.rows} rows, logits of {n}")
+    if rules.masks is not None and (rules.mask_words * 32 < vocab or rules.masks[1] and rules.masks[0] < n):
+        raise ValueError("the mask is smaller than the logits")
+    if out is None:
+        out = torch.empty((n, vocab), dtype=torch.float32, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != torch.float32 or (out.stride(1) != 1 and vocab > 1):
+        raise ValueError("out must be an f32 tensor of the logits' shape with unit-stride rows")
+    if tokens is None and greedy:
+        tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+    if tokens is not None:
+        if tokens.shape != (n,):
+            raise ValueError("one token per row")
+        _i32(tokens)
+        if workspace is None:
+            workspace = logits_workspace(n, logits.device)
+    for t in (out, tokens, workspace, rules):
+        if t is not None and t.device not in (None, logits.device):
+            raise ValueError(f"tensors on {t.device} and {logits.device}")
+    st = (lambda t: t.stride(0) if n > 1 else vocab)
+    L.check(L.lib().mtn_process_logits(_ptr(logits), _dtype_code(logits.dtype), st(logits), n, vocab, rules._ref,
+                                       _ptr(out), st(out), _ptr(tokens), _ptr(workspace),
+                                       0 if workspace is None else workspace.numel(), _stream(stream)))
+    return out, tokens
+
+
 DEV_ERR_TIMEOUT = 4  # a bounded device wait ran out
 
 
