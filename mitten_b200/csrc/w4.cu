@@ -164,6 +164,140 @@ struct W4Params {
   int64_t out_stride;
 };
 
+// ------------------------------------------------------------------ matvec
+//
+// The weights are the A operand of mma.m16n8k16 (16 output rows x 16 k), the
+// x rows its B operand, so up to 8 x rows cost no more than one, and the
+// kernel is bound by the weights' bytes.  A lane's 16-byte vector of a unit
+// is its A fragment of four such products (k in an order of the layout's own,
+// which the x fragments follow): per word and pair of neighbours one shift,
+// one lop3 that masks, flips the sign bit and sets the exponent of 16 --
+// bf16(17 + q / 8) -- and one subtraction of 17, exact.  A group's products
+// add up in f32 and meet the group's scale once, in f32.
+//
+// f32 rows are cut into three bf16 parts of 8 bits each, which hold all 24
+// bits, and multiplied part by part into the same sums.
+//
+// Work.  A cluster of S CTAs takes a contiguous range of row units, each CTA
+// an S-th of k, whose x rows it stages in shared memory once.  Inside the CTA
+// the (row unit, 128 k) steps are laid end to end and each of the 16 warps
+// streams an equal contiguous part of them through a ring of its own, a few
+// steps of asynchronous copies ahead of its products: no barrier until the
+// end, and no warp has more than one step more than another.  With S = 1 a
+// warp stores the units it has whole; the at most two it shares with its
+// neighbours, and with S > 1 every unit, are left in shared memory as partial
+// sums and added at the end in warp order, over the cluster's CTAs in rank
+// order, so results do not depend on timing.
+
+constexpr int kMvWarps = 16;
+constexpr int kMvThreads = kMvWarps * 32;
+constexpr int kXPad = 32;              // elements: rows 64 bytes apart modulo 128, no bank conflicts
+constexpr int kMinUnits = 8;    // row units of a round that the slots of a split have room for at least
+constexpr int kJoinSteps = 16;
+constexpr int kSmemMax = 225 * 1024;
+
+constexpr int mv_units(int parts, int nt) { return parts * nt > 1 ? 2 : 1; }          // kR
+constexpr int mv_depth(int parts, int nt) { return mv_units(parts, nt) > 1 ? 2 : 5; }  // kD
+constexpr int mv_stage(int r, int groups) { return r * (1024 + 32 * groups); }         // bytes of a step
+constexpr int mv_slot(int r, int nt) { return 16 * r * 8 * nt; }                       // floats of a slot
+
+struct MvPlan {
+  int cluster;     // CTAs along k
+  int clusters;
+  int per, extra;  // row units of a cluster; the first `extra` have one more
+  int tile;        // x rows of one pass
+  int units_cap;   // row units of one round
+  int x_stride;    // elements between staged rows
+  int x_vec;       // x rows allow 16-byte loads
+  size_t smem, ring_off, slots_off;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with c = 0.
+__device__ __forceinline__ void mma_bf16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// Neighbours k = 2 p, 2 p + 1 of a word as bf16x2 of q / 8.
+template <int p>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x41884188, 0x6a;" : "=r"(r) : "r"(w >> (4 * p)));  // (a & b) ^ c
+  asm("sub.bf16x2 %0, %0, %1;" : "+r"(r) : "r"(0x41884188u));
+  return r;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// The first `bytes` of 16, zeros for the rest.
+__device__ __forceinline__ void cp_async16_fill(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// f32 at offset `off` of CTA `rank`'s shared memory.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank));
+  return v;
+}
+
+// Three bf16 parts of an f32 value, cut (not rounded) so that no part
+// overflows: hi + mid + lo == x for every finite x (below the range of
+// bf16's subnormals the last bits are lost).
+__device__ __forceinline__ void split3(float x, uint16_t (&h)[3]) {
+  if (!(fabsf(x) < INFINITY)) {  // infinity or NaN: one part
+    h[0] = static_cast<uint16_t>(x != x ? 0x7fc0u : __float_as_uint(x) >> 16);
+    h[1] = h[2] = 0;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t b = __float_as_uint(x) & 0xffff0000u;
+    h[i] = static_cast<uint16_t>(b >> 16);
+    x -= __uint_as_float(b);
+  }
+}
+
 __device__ __forceinline__ void store_out(const W4Params& p, int64_t m, int64_t n, float v) {
   v *= 8.0f;
   if (p.x_scales != nullptr) v *= p.x_scales[m];
@@ -173,32 +307,419 @@ __device__ __forceinline__ void store_out(const W4Params& p, int64_t m, int64_t 
     static_cast<float*>(p.out)[m * p.out_stride + n] = v;
 }
 
-// One warp per output row and x row: lane l takes the words of its row in
-// turn, eight products each.
-__global__ void __launch_bounds__(256) w4_matvec_kernel(const W4Params p) {
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 5;
-  if (row >= p.n) return;
-  const int64_t m = blockIdx.y;
-  const int lane = threadIdx.x & 31;
-  const int64_t kp = pad_k(p.k), ru = row / kRowUnit;
-  const int r = static_cast<int>(row - ru * kRowUnit), g = r & 7;
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(p.packed + ru * (kp / 64) * 32);
-  const uint32_t* sc = p.scales + ru * (kp / p.group) * 8;
-  float acc = 0.0f;
-  for (int64_t c = lane; c * 8 < p.k; c += 32) {  // chunk c: k = 8 c .. 8 c + 7
-    const int64_t unit = c >> 3;
-    const int h = static_cast<int>(c >> 2) & 1, t = static_cast<int>(c) & 3;
-    const uint32_t w = words[(unit * 32 + 4 * g + t) * 4 + (r >> 3) * 2 + h];
-    const uint32_t s2 = sc[(c * 8 / p.group) * 8 + g];
-    float part = 0.0f;
+// Eight consecutive elements of an x row; `vec`: 16-byte loads are aligned.
+template <int kParts>
+__device__ __forceinline__ void load8(const W4Params& p, int64_t at, int64_t k, bool vec, float (&v)[8]) {
+  if (vec && k + 8 <= p.k) {
+    if constexpr (kParts == 3) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + at);
+      const float4 a = q[0], b = q[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else if (p.x_dtype == MTN_DTYPE_BF16) {
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c * 8 + j < p.k)
-        part = fmaf(ld_any(p.x, m * p.x_stride + c * 8 + j, p.x_dtype), static_cast<float>(code_of(w, j)) * 0.125f, part);
-    acc = fmaf(part, __uint_as_float(r >= 8 ? s2 & 0xffff0000u : s2 << 16), acc);
+      for (int i = 0; i < 4; ++i) v[2 * i] = bf2_to_f2(w[i]).x, v[2 * i + 1] = bf2_to_f2(w[i]).y;
+    } else {
+      const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.x) + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __nv_fp8_e4m3 e;
+        e.__x = static_cast<uint8_t>((i < 4 ? a.x : a.y) >> (8 * (i & 3)));
+        v[i] = static_cast<float>(e);
+      }
+    }
+    return;
   }
-  acc = warp_sum(acc);
-  if (lane == 0) store_out(p, m, row, acc);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = k + i < p.k ? ld_any(p.x, at + i, kParts == 3 ? MTN_DTYPE_F32 : p.x_dtype) : 0.0f;
+}
+
+// Copies x rows m0 .. m0 + mt, k0 .. k0 + len, to shared memory as they are
+// (aligned bf16 rows), zeros beyond k; asynchronous.
+__device__ __forceinline__ void copy_rows(const W4Params& p, const MvPlan& plan, uint32_t xs, int64_t m0, int mt,
+                                          int64_t k0, int len) {
+  const uint16_t* x = static_cast<const uint16_t*>(p.x) + m0 * p.x_stride + k0;
+  for (int v = threadIdx.x * 8; v < len; v += kMvThreads * 8) {
+    const int64_t left = (p.k - k0 - v) * 2;
+    const uint32_t bytes = left >= 16 ? 16u : left > 0 ? static_cast<uint32_t>(left) : 0u;
+    const uint16_t* src = bytes > 0 ? x + v : x;
+    for (int m = 0; m < mt; ++m) cp_async16_fill(xs + (m * plan.x_stride + v) * 2, src + m * p.x_stride, bytes);
+  }
+}
+
+// The same through registers, for every other row: f32 cut into three bf16
+// parts, e4m3 exact in bf16, unaligned rows.  kBatch rows are in flight.
+template <int kParts>
+__device__ __forceinline__ void convert_rows(const W4Params& p, const MvPlan& plan, uint16_t* xs, int64_t m0, int mt,
+                                             int64_t k0, int len) {
+  constexpr int kBatch = kParts == 3 ? 2 : 4;
+  for (int e = threadIdx.x * 8; e < len; e += kMvThreads * 8) {
+    for (int mb = 0; mb < mt; mb += kBatch) {
+      float v[kBatch][8];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (mb + b < mt) load8<kParts>(p, (m0 + mb + b) * p.x_stride + k0 + e, k0 + e, plan.x_vec != 0, v[b]);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (mb + b >= mt) continue;
+        uint16_t* dst = xs + (mb + b) * plan.x_stride + e;
+        if constexpr (kParts == 1) {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(f2_to_bf2(v[b][0], v[b][1]), f2_to_bf2(v[b][2], v[b][3]),
+                                                      f2_to_bf2(v[b][4], v[b][5]), f2_to_bf2(v[b][6], v[b][7]));
+        } else {
+          uint16_t h[8][3];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) split3(v[b][j], h[j]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = h[2 * j][q] | static_cast<uint32_t>(h[2 * j + 1][q]) << 16;
+            *reinterpret_cast<uint4*>(dst + q * plan.tile * plan.x_stride) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// kParts: bf16 parts of an x value (1, or 3 for f32).  kNT: 8-row tiles of
+// x.  kR: 16-row units of one step, sharing its x fragments.  kGroups:
+// scale groups in a step of 128 k.  kD: steps loaded ahead.
+template <int kParts, int kNT, int kR, int kGroups, int kD>
+__global__ void __launch_bounds__(kMvThreads, 1) w4_matvec_kernel(const W4Params p, const MvPlan plan) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint16_t* xs = reinterpret_cast<uint16_t*>(smem);
+  float* slots = reinterpret_cast<float*>(smem + plan.slots_off);
+  constexpr int kSlot = mv_slot(kR, kNT);  // [x row][output row]
+  constexpr int kStage = mv_stage(kR, kGroups);
+  static_assert(kD * kStage >= kSlot * 4, "a warp's ring also holds a slot");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int S = plan.cluster;
+  const int rank = S > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int cl = static_cast<int>(blockIdx.x) / S;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * plan.tile;
+  const int mt = static_cast<int>(min(static_cast<int64_t>(plan.tile), p.m - m0));
+  const int ksteps = static_cast<int>(pad_k(p.k) / kKPad);
+  const int runits = static_cast<int>(row_units(p.n));
+  const int cu0 = cl * plan.per + min(cl, plan.extra), cu1 = cu0 + plan.per + (cl < plan.extra ? 1 : 0);
+  const int s0 = rank * ksteps / S, L = (rank + 1) * ksteps / S - s0;
+
+  // The lane's x fragments: row g of each tile, 8 t elements into a half
+  // unit.  Rows beyond the tile read its last row: their sums are not stored.
+  const uint16_t* xf[kNT];
+#pragma unroll
+  for (int j = 0; j < kNT; ++j) xf[j] = xs + min(8 * j + g, mt - 1) * plan.x_stride + 8 * t;
+  const int plane = plan.tile * plan.x_stride;
+
+  uint8_t* ring_ptr = smem + plan.ring_off + warp * (kD * kStage);
+  const uint32_t ring = smem_u32(ring_ptr);
+  const bool direct = kParts == 1 && p.x_dtype == MTN_DTYPE_BF16 && plan.x_vec != 0;
+  const int64_t k0 = static_cast<int64_t>(s0) * kKPad;
+
+  for (int u0 = cu0; u0 < cu1; u0 += plan.units_cap) {
+    const int nu = min(cu1 - u0, plan.units_cap);
+    const int total = nu * L;
+    const int i0 = warp * total / kMvWarps;
+    const int n_items = (warp + 1) * total / kMvWarps - i0;
+    // load cursor and compute cursor: (unit of the round, step of the slice)
+    int lu = L > 0 ? i0 / L : 0, ls = i0 - lu * L;
+    int cu = lu, cs = ls;
+    const uint4* wp[kR];
+    const uint4* sp[kR];
+    auto seek = [&]() {  // an odd last unit reads its first half twice; its rows are not stored
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        const int64_t at = static_cast<int64_t>(min((u0 + lu) * kR + r, runits - 1)) * ksteps + s0 + ls;
+        wp[r] = p.packed + at * 64 + lane;
+        sp[r] = reinterpret_cast<const uint4*>(p.scales) + at * (kGroups * 2) + lane;
+      }
+    };
+    auto load = [&](uint32_t at) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) {
+        cp_async16(at + r * 1024 + lane * 16, wp[r]);
+        cp_async16(at + r * 1024 + 512 + lane * 16, wp[r] + 32);
+        wp[r] += 64;
+        if (lane < 2 * kGroups) cp_async16(at + kR * 1024 + r * (kGroups * 32) + lane * 16, sp[r]);
+        sp[r] += kGroups * 2;
+      }
+      if (++ls == L) {
+        ls = 0;
+        ++lu;
+        seek();
+      }
+    };
+    // x before the weights: behind them it would wait for all their bytes
+    if (u0 == cu0) {
+      if (direct) copy_rows(p, plan, smem_u32(xs), m0, mt, k0, L * kKPad);
+      cp_async_commit();
+    }
+    seek();
+#pragma unroll
+    for (int d = 0; d < kD; ++d) {
+      if (d < n_items) load(ring + d * kStage);
+      cp_async_commit();
+    }
+
+    if (u0 == cu0) {
+      if (!direct) convert_rows<kParts>(p, plan, xs, m0, mt, k0, L * kKPad);
+      cp_async_wait<kD>();  // the copied rows, not the weights behind them
+      __syncthreads();
+    }
+
+    float acc[kR][kNT][4] = {};
+    // The lane holds output rows g, g + 8 of x rows 2 t, 2 t + 1 of each tile.
+    auto leave = [&](float* sl) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sl[(8 * j + 2 * t + (e & 1)) * (16 * kR) + 16 * r + g + 8 * (e >> 1)] = acc[r][j][e];
+            acc[r][j][e] = 0.0f;
+          }
+    };
+    auto finish = [&]() {  // at a unit's end
+      if (S > 1) {
+        leave(slots + (cu + warp) * kSlot);
+      } else if (cu * L < i0) {  // its beginning is the warp before's
+        leave(slots + warp * kSlot);
+      } else {
+#pragma unroll
+        for (int r = 0; r < kR; ++r)
+#pragma unroll
+          for (int j = 0; j < kNT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int m = 8 * j + 2 * t + (e & 1);
+              const int64_t n = static_cast<int64_t>((u0 + cu) * kR + r) * 16 + g + 8 * (e >> 1);
+              if (m < mt && n < p.n) store_out(p, m0 + m, n, acc[r][j][e]);
+              acc[r][j][e] = 0.0f;
+            }
+      }
+    };
+    uint32_t at = ring;
+    for (int i = 0; i < n_items; ++i) {
+      cp_async_wait<kD - 1>();
+      __syncwarp();  // the scales came through other lanes
+      const int xo = cs * kKPad;
+      float cg[kR][kNT][4];
+      uint4 w[kR];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {  // 32 k: half h & 1 of unit h >> 1
+        constexpr int kPer = 4 / kGroups;  // halves in a group
+        if ((h & 1) == 0) {
+#pragma unroll
+          for (int r = 0; r < kR; ++r) w[r] = lds16(at + r * 1024 + (h >> 1) * 512 + lane * 16);
+        }
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+          uint4 xv[kNT];
+#pragma unroll
+          for (int j = 0; j < kNT; ++j) xv[j] = *reinterpret_cast<const uint4*>(xf[j] + q * plane + xo + 32 * h);
+#pragma unroll
+          for (int r = 0; r < kR; ++r) {
+            const uint32_t lo = h & 1 ? w[r].y : w[r].x, hi = h & 1 ? w[r].w : w[r].z;
+            const uint32_t a0 = code_pair<0>(lo), a1 = code_pair<0>(hi), a2 = code_pair<1>(lo), a3 = code_pair<1>(hi);
+            const uint32_t b0 = code_pair<2>(lo), b1 = code_pair<2>(hi), b2 = code_pair<3>(lo), b3 = code_pair<3>(hi);
+#pragma unroll
+            for (int j = 0; j < kNT; ++j) {
+              if (h % kPer == 0 && q == 0)
+                mma_bf16_zero(cg[r][j], a0, a1, a2, a3, xv[j].x, xv[j].y);
+              else
+                mma_bf16(cg[r][j], a0, a1, a2, a3, xv[j].x, xv[j].y);
+              mma_bf16(cg[r][j], b0, b1, b2, b3, xv[j].z, xv[j].w);
+            }
+          }
+        }
+        if ((h + 1) % kPer == 0) {  // end of a group
+#pragma unroll
+          for (int r = 0; r < kR; ++r) {
+            const uint32_t s2 = lds4(at + kR * 1024 + (r * kGroups + h / kPer) * 32 + g * 4);
+            const float slo = __uint_as_float(s2 << 16), shi = __uint_as_float(s2 & 0xffff0000u);
+#pragma unroll
+            for (int j = 0; j < kNT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[r][j][e] = fmaf(cg[r][j][e], e < 2 ? slo : shi, acc[r][j][e]);
+          }
+        }
+      }
+      // every lane has read the stage: refill it
+      __syncwarp();
+      if (i + kD < n_items) load(at);
+      cp_async_commit();
+      at = at + kStage == ring + kD * kStage ? ring : at + kStage;
+      if (++cs == L) {
+        finish();
+        cs = 0;
+        ++cu;
+      }
+    }
+    if (n_items > 0 && cs != 0) {  // the unit goes on in the next warp
+      if (S > 1)
+        leave(slots + (cu + warp) * kSlot);
+      else if (cu * L < i0)
+        leave(slots + warp * kSlot);
+      else
+        leave(reinterpret_cast<float*>(ring_ptr));  // the ring is empty by now
+    }
+
+    constexpr int kUnitRows = 16 * kR;
+    if (S > 1) {
+      // Join the warps' slots of each unit into the space of the rings, then
+      // those of the cluster's CTAs.
+      float* part = reinterpret_cast<float*>(smem + plan.ring_off);
+      __syncthreads();
+      for (int q = warp; q < nu; q += kMvWarps) {
+        int wa = 0, wb = -1;  // first and last warp with a step of unit q
+        if (L > 0) {
+          wa = ((q * L + 1) * kMvWarps - 1) / total;
+          wb = ((q + 1) * L * kMvWarps - 1) / total;
+        }
+        for (int i = lane; i < mt * kUnitRows; i += 32) {
+          float v = 0.0f;
+          for (int w = wa; w <= wb; ++w)
+            if (w * total / kMvWarps != (w + 1) * total / kMvWarps) v += slots[(q + w) * kSlot + i];
+          part[q * kSlot + i] = v;
+        }
+      }
+      cluster_sync();
+      const uint32_t part_at = smem_u32(part);
+      const int per_unit = mt * kUnitRows;
+      for (int i = rank * kMvThreads + tid; i < nu * per_unit; i += S * kMvThreads) {
+        const int q = i / per_unit, off = i - q * per_unit;
+        float v[8];
+#pragma unroll
+        for (int rk = 0; rk < 8; ++rk)
+          if (rk < S) v[rk] = ld_cluster(part_at + (q * kSlot + off) * 4, rk);
+        float sum = 0.0f;
+#pragma unroll
+        for (int rk = 0; rk < 8; ++rk)
+          if (rk < S) sum += v[rk];
+        const int64_t n = static_cast<int64_t>(u0 + q) * kUnitRows + off % kUnitRows;
+        if (n < p.n) store_out(p, m0 + off / kUnitRows, n, sum);
+      }
+      cluster_sync();
+    } else {
+      // Join a unit that begins in this warp and goes on in the next ones.
+      __syncthreads();
+      const int i1 = i0 + n_items, q = i1 / L;
+      if (n_items > 0 && i1 != q * L && q * L >= i0) {
+        const float* tail = reinterpret_cast<const float*>(ring_ptr);
+        for (int i = lane; i < mt * kUnitRows; i += 32) {
+          float v = tail[i];
+          for (int z = warp + 1; z < kMvWarps && z * total / kMvWarps < (q + 1) * L; ++z)
+            if (z * total / kMvWarps != (z + 1) * total / kMvWarps) v += slots[z * kSlot + i];
+          const int64_t n = static_cast<int64_t>(u0 + q) * kUnitRows + i % kUnitRows;
+          if (n < p.n) store_out(p, m0 + i / kUnitRows, n, v);
+        }
+      }
+      if (u0 + nu < cu1) __syncthreads();
+    }
+  }
+}
+
+using MvKernel = void (*)(const W4Params, const MvPlan);
+
+template <int kParts, int kNT>
+MvKernel mv_kernel(int group) {
+  constexpr int kR = mv_units(kParts, kNT), kD = mv_depth(kParts, kNT);
+  switch (group) {
+    case 32: return w4_matvec_kernel<kParts, kNT, kR, 4, kD>;
+    case 64: return w4_matvec_kernel<kParts, kNT, kR, 2, kD>;
+    default: return w4_matvec_kernel<kParts, kNT, kR, 1, kD>;
+  }
+}
+
+// Clusters of `size` CTAs that the device holds at once (one CTA per SM).
+int max_clusters(int size) {
+  constexpr int kDevices = 64;
+  static int cached[kDevices][4] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return std::max(1, 128 / size);
+  const int slot = size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3;
+  if (cached[dev][slot] == 0) {
+    int n = sm_count();
+    if (size > 1) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(size));
+      cfg.blockDim = dim3(kMvThreads);
+      cfg.dynamicSmemBytes = kSmemMax;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      auto kern = mv_kernel<1, 1>(128);
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax)) !=
+              cudaSuccess ||
+          cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = std::max(1, 128 / size);
+      }
+    }
+    cached[dev][slot] = n;
+  }
+  return cached[dev][slot];
+}
+
+// The x rows of one pass and the split of k: as many rows (up to 16) as the
+// slices of a cluster of at most 8 CTAs can hold in shared memory, then the
+// split whose CTAs have the fewest steps, a join of slots counted as
+// kJoinSteps of them.
+MvPlan mv_plan(int64_t m, int64_t n, int64_t k, int group, int parts) {
+  const int ksteps = static_cast<int>(pad_k(k) / kKPad);
+  MvPlan pl{};
+  pl.tile = static_cast<int>(std::min<int64_t>(m, 16));
+  int nt, r;
+  size_t ring, slot;
+  auto sizes = [&]() {
+    nt = pl.tile > 8 ? 2 : 1;
+    r = mv_units(parts, nt);
+    ring = static_cast<size_t>(kMvWarps) * mv_depth(parts, nt) * mv_stage(r, kKPad / group);
+    slot = static_cast<size_t>(mv_slot(r, nt)) * 4;
+  };
+  auto x_bytes = [&](int s) {
+    const size_t b = static_cast<size_t>(parts) * pl.tile * ((ksteps + s - 1) / s * kKPad + kXPad) * 2;
+    return (b + 127) / 128 * 128;
+  };
+  // slots that fit beside the rest: one a warp, and with a split one more for every row unit of a round
+  auto fits = [&](int s) { return x_bytes(s) + ring + (kMvWarps + (s > 1 ? kMinUnits : 0)) * slot <= kSmemMax; };
+  sizes();
+  while (pl.tile > 1 && !fits(8)) {
+    pl.tile = (pl.tile + 1) / 2;
+    sizes();
+  }
+  const int64_t units = (row_units(n) + r - 1) / r;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= 8; s *= 2) {
+    if (!fits(s)) continue;
+    const int64_t c = std::min<int64_t>(units, max_clusters(s));
+    const int64_t per = (units + c - 1) / c;
+    // a round's units: slots for them and for the warps, and the joined units in the rings
+    const int64_t room =
+        std::min(static_cast<int64_t>((kSmemMax - x_bytes(s) - ring) / slot) - kMvWarps, static_cast<int64_t>(ring / slot));
+    const int64_t cap = s == 1 ? 4096 : room;  // 4096: steps x warps stay within 32 bits
+    const int64_t rounds = (per + cap - 1) / cap;
+    const int64_t cost = per * ((ksteps + s - 1) / s) + (s == 1 ? 0 : rounds * kJoinSteps);
+    if (cost < best) {
+      best = cost;
+      pl.cluster = s;
+      pl.clusters = static_cast<int>(c);
+      pl.per = static_cast<int>(units / c);
+      pl.extra = static_cast<int>(units % c);
+      pl.units_cap = static_cast<int>((per + rounds - 1) / rounds);
+    }
+  }
+  pl.x_stride = (ksteps + pl.cluster - 1) / pl.cluster * kKPad + kXPad;
+  pl.ring_off = x_bytes(pl.cluster);
+  pl.slots_off = pl.ring_off + ring;
+  pl.smem = pl.slots_off + (kMvWarps + (pl.cluster > 1 ? pl.units_cap : 0)) * slot;
+  return pl;
 }
 
 int check_sizes(const char* who, int64_t n, int64_t k, int32_t group) {
@@ -287,8 +808,29 @@ int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float*
   MTN_CHECK_ARG(out != x, "mtn_w4_matvec: out overlaps x");
   mtn::W4Params p{x, x_dtype, x_stride, x_scales, n_rows, static_cast<const uint4*>(packed),
                   static_cast<const uint32_t*>(scales), n, k, group, out, out_dtype, out_stride};
-  const dim3 grid(static_cast<unsigned>((n + 7) / 8), static_cast<unsigned>(n_rows));
-  mtn::w4_matvec_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const int parts = x_dtype == MTN_DTYPE_F32 ? 3 : 1;
+  mtn::MvPlan plan = mtn::mv_plan(n_rows, n, k, group, parts);
+  const int elem = x_dtype == MTN_DTYPE_F32 ? 4 : x_dtype == MTN_DTYPE_BF16 ? 2 : 1;
+  const int64_t vec = elem == 1 ? 8 : 16;  // bytes of one vector load
+  plan.x_vec = reinterpret_cast<uintptr_t>(x) % vec == 0 && (n_rows == 1 || x_stride * elem % vec == 0);
+  const bool two = plan.tile > 8;
+  const mtn::MvKernel kern = parts == 1 ? (two ? mtn::mv_kernel<1, 2>(group) : mtn::mv_kernel<1, 1>(group))
+                                        : (two ? mtn::mv_kernel<3, 2>(group) : mtn::mv_kernel<3, 1>(group));
+  MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(mtn::kSmemMax)),
+               "mtn_w4_matvec");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.clusters * plan.cluster),
+                     static_cast<unsigned>((n_rows + plan.tile - 1) / plan.tile));
+  cfg.blockDim = dim3(mtn::kMvThreads);
+  cfg.dynamicSmemBytes = plan.smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(plan.cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MTN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, plan), "w4_matvec_kernel");
   return mtn::check_launch("w4_matvec_kernel");
 }
 
