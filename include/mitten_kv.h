@@ -454,11 +454,17 @@ typedef struct {
  * row's first strict maximum, as mtn_argmax_rows gives it (a row whose mask
  * leaves nothing gives 0).  workspace: for tokens only,
  * mtn_process_logits_workspace_bytes(n_rows) bytes, 8-byte aligned, zeroed
- * once before first use and left zeroed by every call, one stream at a time. */
+ * once before first use and left zeroed by every call, one stream at a time.
+ * scratch: for a history or biases only,
+ * mtn_process_logits_scratch_bytes(n_rows, n_hist, n_bias) bytes, 8-byte
+ * aligned, any contents, one stream at a time.  Rows of an index pointer that
+ * falls share list entries; then the rows that share them are undefined too. */
 MTN_API size_t mtn_process_logits_workspace_bytes(int64_t n_rows);
+MTN_API size_t mtn_process_logits_scratch_bytes(int64_t n_rows, int64_t n_hist, int64_t n_bias);
 MTN_API int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, int64_t n_rows, int64_t vocab,
                                const mtn_logits_rules* rules, float* out, int64_t out_stride, int32_t* tokens,
-                               void* workspace, size_t workspace_bytes, void* stream);
+                               void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                               void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Host mirror: page allocator (kv_pool.rs:4-69) + refcount extension       */

@@ -161,7 +161,9 @@ SIGNATURES: dict[str, tuple] = {
                                   C.c_void_p]),
     "mtn_process_logits_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "mtn_process_logits": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.POINTER(LogitsRules),
-                                     C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+                                     C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p,
+                                     C.c_size_t, C.c_void_p]),
+    "mtn_process_logits_scratch_bytes": (C.c_size_t, [C.c_int64] * 3),
     # host mirror: page pool
     "mtn_page_pool_create": (C.c_int, [C.c_int64, C.c_int32, C.POINTER(C.c_void_p)]),
     "mtn_page_pool_destroy": (None, [C.c_void_p]),

@@ -12,37 +12,66 @@
 // token of the processed row: its first strict maximum (NaN never wins, a
 // row of nothing but -inf gives 0, as scheduler.rs:187-199).
 //
-// One CTA per (row, chunk of the vocabulary).  It counts the row's history
-// tokens that fall into its chunk in shared memory (integer atomics, so the
-// counts do not depend on their order) and marks the touched ones in a
-// bitmap, then passes over its logits once, 16 bytes a load and four loads in
-// flight, the first four already before the counting; only touched elements
-// look their count up.  The chunks of a row join their maxima as 64-bit keys
-// (value, then lowest index) with an atomic maximum; the last chunk to arrive
-// writes the token and leaves the workspace zeroed.
+// Two launches.  sort_rules_kernel, one CTA per row, sorts the row's history
+// and biases by the chunk of the vocabulary they fall into (a counting sort;
+// the order inside a chunk does not matter).  process_logits_kernel, one CTA
+// per (row, chunk), passes over the logits with the mask alone, 16 bytes a
+// load; that pass is bound by memory and needs nothing of the first kernel,
+// which therefore runs beside it (programmatic dependent launch).  Then it
+// waits, counts its entries in a table in shared memory (integer atomics, so
+// nothing depends on their order) and applies penalties and biases to the
+// original logits, the first entry to claim a token doing its work; a thread
+// whose maximum is a touched element looks its elements over again.  The
+// chunks of a row join their maxima as 64-bit keys (value, then lowest index)
+// with an atomic maximum; the last one to arrive writes the token and leaves
+// the workspace zeroed.
+//
+// Not kept, for 64 x 152064 with everything on: every chunk counting over the
+// whole history (50 us: most warp steps met a hit for a lane or two), counting
+// over a cluster's distributed shared memory (56-70 us: a frequent token's
+// remote atomics queue up), one CTA per row making a list of different tokens
+// in a hash table (45 us; 170 us for 128 x 256000, where a row's 13 k different
+// tokens keep one SM busy for 100 us).
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace mtn {
 namespace {
 
 constexpr int kLogitsThreads = 256;
-// Elements of a chunk: large ones re-read a row's history less often, small
-// ones spread few rows over the SMs.
-constexpr int kChunkLarge = 8192, kChunkSmall = 2048;
-constexpr int kBatchVecs = 4;            // 16-byte loads of a thread in flight
-constexpr uint32_t kSeen = 0x80000000u;  // in the history at all; the low bits count the generated part
+constexpr int kLogitsResident = 4;  // CTAs an SM holds, by registers
+constexpr int kChunkStep = 1024, kChunkMax = 32768;
+constexpr int kChunkMaxRuled = 8192;  // tables of 32 KB
+constexpr int kChunkFixed = 2048;
+constexpr int kBatchVecs = 4;         // 16-byte loads of a thread ahead of the ones in work
+constexpr int kSortThreads = 1024;
+constexpr int kBuckets = 512;         // a row's chunks, or groups of 2^k of them
+constexpr uint32_t kGenerated = 0x80000000u;
+
+// Scratch between the two kernels: the entries of each list, sorted by bucket
+// within a row, a row's from its index pointer on, and where the buckets begin.
+struct SortedRules {
+  uint2* bias;          // token, index in the row's list
+  uint32_t* hist;       // token | kGenerated
+  int32_t* hist_starts;  // [rows][kBuckets + 1]
+  int32_t* bias_starts;
+};
 
 struct LogitsParams {
   const void* logits;
   int64_t row_stride;
   int64_t vocab;
   mtn_logits_rules r;
+  SortedRules sorted;
   float* out;
   int64_t out_stride;
   int32_t* tokens;
   unsigned long long* keys;  // [rows] maxima, then [rows] arrival counters
   int64_t n_rows;
-  int chunks, chunk;
+  int chunks, size;  // chunks a row, elements of a chunk
+  int elem;          // bytes of a logit
+  int bucket_shift;  // log2 of the chunks of a bucket
   int* err;
 };
 
@@ -58,42 +87,102 @@ __device__ __forceinline__ void row_range(const int32_t* indptr, int64_t r, int6
   }
 }
 
+// Elements of row `row` before the first that a 16-byte load may start at.
+// Chunk 0 of a row has them and the `size` elements behind them.
+__device__ __forceinline__ int row_head(const LogitsParams& p, int row) {
+  const uint64_t at = reinterpret_cast<uintptr_t>(p.logits) + row * p.row_stride * p.elem;
+  return static_cast<int>((16u - (static_cast<uint32_t>(at) & 15u)) % 16u) / p.elem;
+}
+
+// One row's list, tokens[beg .. end), counted and placed by bucket; place(i, t,
+// to) stores entry i.  All threads of the CTA.
+template <typename F>
+__device__ __forceinline__ void sort_list(const LogitsParams& p, int row, int head, const int32_t* tokens, int64_t beg,
+                                          int64_t end, int32_t* starts, int* count, F place) {
+  constexpr int kAhead = 4;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const uint32_t vocab = static_cast<uint32_t>(p.vocab);
+  auto bucket_of = [&](int32_t t) {
+    return static_cast<int>(static_cast<uint32_t>(max(t - head, 0)) / static_cast<uint32_t>(p.size)) >> p.bucket_shift;
+  };
+  auto each = [&](auto f) {
+    for (int64_t i = beg + tid; i < end; i += kAhead * kSortThreads) {
+      int32_t t[kAhead];
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) t[b] = i + b * kSortThreads < end ? tokens[i + b * kSortThreads] : -1;
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b)
+        if (i + b * kSortThreads < end) f(i + b * kSortThreads, t[b]);
+    }
+  };
+  if (tid < kBuckets) count[tid] = 0;
+  __syncthreads();
+  each([&](int64_t, int32_t t) {
+    if (static_cast<uint32_t>(t) < vocab)
+      atomicAdd(&count[bucket_of(t)], 1);
+    else
+      record_error(p.err, kDevErrBadLogitRule, row);
+  });
+  __syncthreads();
+  if (tid < 32) {  // exclusive sums, 16 buckets a lane
+    constexpr int kPer = kBuckets / 32;
+    int sum = 0;
+    for (int i = 0; i < kPer; ++i) sum += count[lane * kPer + i];
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    int run = upto - sum;
+    for (int i = 0; i < kPer; ++i) {
+      const int n = count[lane * kPer + i];
+      count[lane * kPer + i] = run;
+      run += n;
+    }
+    if (lane == 31) starts[kBuckets] = upto;
+  }
+  __syncthreads();
+  if (tid < kBuckets) starts[tid] = count[tid];
+  __syncthreads();
+  each([&](int64_t i, int32_t t) {
+    if (static_cast<uint32_t>(t) < vocab) place(i, t, beg + atomicAdd(&count[bucket_of(t)], 1));
+  });
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_rules_kernel(const LogitsParams p) {
+  __shared__ int count[kBuckets];
+  // the next kernel's first pass reads nothing of this one
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int row = static_cast<int>(blockIdx.x), head = row_head(p, row);
+  const int64_t at = static_cast<int64_t>(row) * (kBuckets + 1);
+  if (p.r.hist_indptr != nullptr) {
+    int64_t beg, end;
+    row_range(p.r.hist_indptr, row, p.r.n_hist, beg, end, p.err);
+    const int64_t gen = beg + (p.r.prompt_lens != nullptr ? max(p.r.prompt_lens[row], 0) : 0);
+    sort_list(p, row, head, p.r.hist_tokens, beg, end, p.sorted.hist_starts + at, count,
+              [&](int64_t i, int32_t t, int64_t to) {
+                p.sorted.hist[to] = static_cast<uint32_t>(t) | (i >= gen ? kGenerated : 0u);
+              });
+    __syncthreads();
+  }
+  if (p.r.bias_indptr != nullptr) {
+    int64_t beg, end;
+    row_range(p.r.bias_indptr, row, p.r.n_bias, beg, end, p.err);
+    sort_list(p, row, head, p.r.bias_tokens, beg, end, p.sorted.bias_starts + at, count,
+              [&](int64_t i, int32_t t, int64_t to) {
+                p.sorted.bias[to] = make_uint2(static_cast<uint32_t>(t), static_cast<uint32_t>(i - beg));
+              });
+  }
+}
+
 // Order-preserving key of a processed logit: larger values first, then the
 // lower index.  0 for what never wins (-inf, NaN).  x + 0 turns -0 into +0.
-__device__ __forceinline__ unsigned long long arg_key(float x, int64_t v) {
+__device__ __forceinline__ unsigned long long arg_key(float x, int v) {
   if (!(x > -INFINITY)) return 0ull;
   const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
   const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
   return static_cast<unsigned long long>(o) << 32 | (0xffffffffu - static_cast<uint32_t>(v));
-}
-
-// Calls f(position, token) for entries [beg, end) of an int32 list, 16 bytes
-// a load where the list's address allows.
-template <typename F>
-__device__ __forceinline__ void for_tokens(const int32_t* list, int64_t beg, int64_t end, F f) {
-  const int tid = threadIdx.x;
-  const int64_t head = min(end, beg + static_cast<int64_t>((0u - (reinterpret_cast<uintptr_t>(list + beg) >> 2)) & 3u));
-  if (beg + tid < head) f(beg + tid, list[beg + tid]);
-  const int4* vec = reinterpret_cast<const int4*>(list + head);
-  const int n = static_cast<int>((end - head) >> 2);
-  for (int i = tid; i < n; i += 2 * kLogitsThreads) {
-    const bool two = i + kLogitsThreads < n;
-    const int4 a = vec[i], b = two ? vec[i + kLogitsThreads] : a;
-    const int64_t at = head + 4 * static_cast<int64_t>(i);
-    f(at, a.x), f(at + 1, a.y), f(at + 2, a.z), f(at + 3, a.w);
-    if (two) {
-      const int64_t bt = at + 4 * kLogitsThreads;
-      f(bt, b.x), f(bt + 1, b.y), f(bt + 2, b.z), f(bt + 3, b.w);
-    }
-  }
-  const int64_t rest = head + 4 * static_cast<int64_t>(n) + tid;
-  if (rest < end) f(rest, list[rest]);
-}
-
-// Bits i .. i + 31 of a bit array of n words (zeros behind its end are not needed).
-__device__ __forceinline__ uint32_t bits_at(const uint32_t* words, int64_t n, int64_t i) {
-  const int64_t w = i >> 5;
-  return __funnelshift_r(words[w], words[min(w + 1, n - 1)], static_cast<uint32_t>(i) & 31u);
 }
 
 template <typename T>
@@ -113,161 +202,197 @@ __device__ __forceinline__ float ld_logit(const T* p) {
   else return *p;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads) process_logits_kernel(const LogitsParams p) {
+// kHist, kBias: a history, biases are given, and sort_rules_kernel went before.
+template <typename T, bool kHist, bool kBias>
+__global__ void __launch_bounds__(kLogitsThreads, kLogitsResident) process_logits_kernel(const LogitsParams p) {
   extern __shared__ __align__(16) uint32_t smem[];
   constexpr int kN = Vec<T>::kN;
-  const int row = static_cast<int>(blockIdx.x) / p.chunks;
-  const int chunk = static_cast<int>(blockIdx.x) - row * p.chunks;
+  constexpr bool kRules = kHist || kBias;
   const int tid = threadIdx.x;
+  const int row = static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.chunks));
+  const int chunk = static_cast<int>(blockIdx.x - static_cast<uint32_t>(row) * p.chunks), vocab = static_cast<int>(p.vocab);
   const T* in = static_cast<const T*>(p.logits) + row * p.row_stride;
   float* out = p.out + row * p.out_stride;
-  // Chunks begin where a 16-byte load may: `head` elements into the row.
-  const int head = static_cast<int>((0u - (reinterpret_cast<uintptr_t>(in) / sizeof(T))) & (kN - 1u));
-  const bool vec = ((reinterpret_cast<uintptr_t>(out + head)) & 15u) == 0;
-  const int64_t v0 = chunk == 0 ? 0 : static_cast<int64_t>(chunk) * p.chunk + head;
-  const int64_t v1 = chunk == p.chunks - 1 ? p.vocab : min(p.vocab, static_cast<int64_t>(chunk + 1) * p.chunk + head);
-  const int nv = static_cast<int>(max(v1 - v0, static_cast<int64_t>(0)));
-  // vectors: elements body .. body + kN * nvec of the row; the rest one by one
-  const int64_t body = chunk == 0 ? min(static_cast<int64_t>(head), v1) : v0;
-  const int nvec = vec && v1 > body ? static_cast<int>((v1 - body) / kN) : 0;
+  // Chunks begin where a 16-byte load may: `head` elements into the row; the
+  // first one has the elements before that too.
+  const int head = row_head(p, row);
+  const bool vec = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out + head)) & 15u) == 0;
+  auto start_of = [&](int c) {
+    return c == 0 ? 0 : c >= p.chunks ? vocab : static_cast<int>(min(static_cast<int64_t>(vocab), static_cast<int64_t>(c) * p.size + head));
+  };
+  const int v0 = start_of(chunk), nv = start_of(chunk + 1) - v0;
+  in += v0;
+  out += v0;  // from here on elements count from the chunk's first
+  const int body = chunk == 0 ? min(head, nv) : 0;  // vectors: body .. body + kN * nvec; the rest one by one
+  const int nvec = vec ? (nv - body) / kN : 0;
   const uint4* vin = reinterpret_cast<const uint4*>(in + body);
+  float4* vout = reinterpret_cast<float4*>(out + body);
 
-  Vec<T> x[kBatchVecs];
-#pragma unroll
-  for (int b = 0; b < kBatchVecs; ++b)
-    if (tid + b * kLogitsThreads < nvec) x[b].w = vin[tid + b * kLogitsThreads];
-
-  // shared memory: touched bits of the chunk's words, then counts, then bias entries
-  const int64_t w0 = v0 >> 5;
-  const int nwords = p.chunk / 32 + 2;
-  const bool hist = p.r.hist_indptr != nullptr, biased = p.r.bias_indptr != nullptr, rules = hist || biased;
-  uint32_t* touched = smem;
-  uint32_t* count = smem + (nwords + 3) / 4 * 4;
-  uint32_t* bias = count + (hist ? p.chunk + 8 : 0);
-  int64_t bias_beg = 0;
-  if (rules) {
-    int64_t hbeg = 0, hend = 0, bend = 0;
-    if (hist) row_range(p.r.hist_indptr, row, p.r.n_hist, hbeg, hend, p.err);
-    if (biased) row_range(p.r.bias_indptr, row, p.r.n_bias, bias_beg, bend, p.err);
-    const int words = static_cast<int>(bias - touched) + (biased ? p.chunk + 8 : 0);
-    for (int i = tid; i < words / 4; i += kLogitsThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    auto slot = [&](int32_t t, int& k) {  // the token's place in the chunk
-      if (t < 0 || t >= p.vocab) {
-        record_error(p.err, kDevErrBadLogitRule, row);
-        return false;
-      }
-      k = static_cast<int>(t - v0);
-      if (t < v0 || t >= v1) return false;
-      const int64_t w = (t >> 5) - w0;
-      const uint32_t bit = 1u << (t & 31);
-      if (!(touched[w] & bit)) atomicOr(&touched[w], bit);
-      return true;
-    };
-    if (hist) {
-      const int64_t gen = hbeg + (p.r.prompt_lens != nullptr ? max(p.r.prompt_lens[row], 0) : 0);
-      for_tokens(p.r.hist_tokens, hbeg, hend, [&](int64_t i, int32_t t) {
-        int k;
-        if (!slot(t, k)) return;
-        if (i >= gen)
-          atomicAdd(&count[k], 1u);
-        if (!(count[k] & kSeen)) atomicOr(&count[k], kSeen);
-      });
-    }
-    if (biased)
-      for_tokens(p.r.bias_tokens, bias_beg, bend, [&](int64_t i, int32_t t) {
-        int k;
-        if (slot(t, k)) atomicMax(&bias[k], static_cast<uint32_t>(i - bias_beg + 1));
-      });
-  }
-  const float rep = p.r.repetition != nullptr ? p.r.repetition[row] : 1.0f;
-  const float freq = p.r.frequency != nullptr ? p.r.frequency[row] : 0.0f;
-  const float pres = p.r.presence != nullptr ? p.r.presence[row] : 0.0f;
+  // The mask's words from the chunk's first element's on, and that element's bit.
   const uint32_t* mask = nullptr;
-  const int64_t mask_words = (p.vocab + 31) >> 5;
+  const int mask_bit = v0 & 31, mask_last = ((vocab - 1) >> 5) - (v0 >> 5);
   if (p.r.mask != nullptr) {
     const int mr = p.r.mask_rows != nullptr ? p.r.mask_rows[row] : row;
     if (mr >= 0 && mr < p.r.n_masks)
-      mask = p.r.mask + mr * p.r.mask_stride;
+      mask = p.r.mask + mr * p.r.mask_stride + (v0 >> 5);
     else if (mr != -1 && tid == 0)
       record_error(p.err, kDevErrBadLogitRule, row);
   }
-  if (rules) __syncthreads();
+  auto allowed = [&](int k) { return mask == nullptr || (mask[(k + mask_bit) >> 5] >> ((k + mask_bit) & 31) & 1u) != 0; };
 
-  auto ruled = [&](float y, int64_t v) {  // a touched element's penalties and bias
-    const int k = static_cast<int>(v - v0);
-    if (hist && count[k] != 0) {
-      const uint32_t c = count[k] & ~kSeen;
-      y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-      y = __fsub_rn(y, __fmul_rn(freq, static_cast<float>(c)));
-      if (c != 0) y = __fsub_rn(y, pres);
-    }
-    if (biased && bias[k] != 0) y = __fadd_rn(y, p.r.bias_values[bias_beg + bias[k] - 1]);
-    return y;
-  };
-  // A thread sees rising indices, so a strict comparison keeps the first maximum.
+  // A thread sees rising places, so a strict comparison keeps the first maximum.
   float best = -INFINITY;
-  int64_t best_v = 0;
-  auto scalar = [&](int64_t v) {
-    float y = ld_logit(in + v);
-    if (rules && touched[(v >> 5) - w0] >> (v & 31) & 1u) y = ruled(y, v);
-    if (mask != nullptr && !(mask[v >> 5] >> (v & 31) & 1u)) y = -INFINITY;
-    out[v] = y;
-    if (y > best) best = y, best_v = v;
+  int best_k = 0;
+  auto scalar = [&](int k) {
+    float y = ld_logit(in + k);
+    if (!allowed(k)) y = -INFINITY;
+    out[k] = y;
+    if (y > best) best = y, best_k = k;
   };
-  if (!vec) {
-    for (int i = tid; i < nv; i += kLogitsThreads) scalar(v0 + i);
-  } else {
-    if (v0 + tid < body) scalar(v0 + tid);
-    for (int base = tid; base < nvec; base += kBatchVecs * kLogitsThreads) {
-      uint32_t allow[kBatchVecs];
-#pragma unroll
-      for (int b = 0; b < kBatchVecs; ++b) {
-        const int i = base + b * kLogitsThreads;
-        allow[b] = ~0u;
-        if (mask != nullptr && i < nvec) allow[b] = bits_at(mask, mask_words, body + static_cast<int64_t>(i) * kN);
+  if (vec) {
+    if (tid < body) scalar(tid);
+    // A step of 256 vectors is a whole number of mask words, so a thread's
+    // bits lie at the same place of a word every time.
+    const int bit = body + tid * kN + mask_bit, sh = bit & 31;
+    const uint32_t* mw = mask + (bit >> 5);
+    constexpr int kWords = kLogitsThreads * kN / 32;
+    const int wlast = mask_last - (bit >> 5);
+    Vec<T> x[kBatchVecs];
+    uint32_t m[kBatchVecs];
+    auto load = [&](int b, int i, int step) {
+      if (i < nvec) {
+        x[b].w = vin[i];
+        m[b] = mask != nullptr ? mw[step * kWords] : ~0u;
       }
+    };
+#pragma unroll
+    for (int b = 0; b < kBatchVecs; ++b) load(b, tid + b * kLogitsThreads, b);
+    for (int i = tid, step = 0; i < nvec; i += kBatchVecs * kLogitsThreads, step += kBatchVecs) {
 #pragma unroll
       for (int b = 0; b < kBatchVecs; ++b) {
-        const int i = base + b * kLogitsThreads;
-        if (i >= nvec) break;
-        const int64_t v = body + static_cast<int64_t>(i) * kN;
-        float y[kN];
+        const int j = i + b * kLogitsThreads;
+        if (j < nvec) {
+          uint32_t allow = ~0u;
+          if (mask != nullptr) {
+            allow = m[b] >> sh;
+            if (sh > 32 - kN) allow |= mw[min((step + b) * kWords + 1, wlast)] << (32 - sh);
+          }
+          float y[kN];
 #pragma unroll
-        for (int e = 0; e < kN; ++e) y[e] = x[b].get(e);
-        if (rules) {
-          const uint32_t hit = bits_at(touched, nwords, v - (w0 << 5)) & ((1u << kN) - 1u);
-          if (hit != 0) {
+          for (int e = 0; e < kN; ++e) y[e] = allow & (1u << e) ? x[b].get(e) : -INFINITY;
+          load(b, j + kBatchVecs * kLogitsThreads, step + b + kBatchVecs);
 #pragma unroll
-            for (int e = 0; e < kN; ++e)
-              if (hit >> e & 1u) y[e] = ruled(y[e], v + e);
+          for (int e = 0; e < kN; e += 4) vout[j * (kN / 4) + e / 4] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+          float top = y[0];
+#pragma unroll
+          for (int e = 1; e < kN; ++e) top = fmaxf(top, y[e]);
+          if (top > best) {
+            best = top;
+#pragma unroll
+            for (int e = kN - 1; e >= 0; --e)
+              if (y[e] == top) best_k = body + j * kN + e;
           }
         }
-#pragma unroll
-        for (int e = 0; e < kN; ++e)
-          if (!(allow[b] >> e & 1u)) y[e] = -INFINITY;
-        float top = y[0];
-#pragma unroll
-        for (int e = 1; e < kN; ++e) top = fmaxf(top, y[e]);
-        if (top > best) {
-          best = top;
-#pragma unroll
-          for (int e = kN - 1; e >= 0; --e)
-            if (y[e] == top) best_v = v + e;
-        }
-#pragma unroll
-        for (int e = 0; e < kN; e += 4)
-          *reinterpret_cast<float4*>(out + v + e) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-        const int next = i + kBatchVecs * kLogitsThreads;
-        if (next < nvec) x[b].w = vin[next];
       }
     }
-    const int64_t rest = body + static_cast<int64_t>(nvec) * kN + tid;
-    if (rest < v1) scalar(rest);
+    const int rest = body + nvec * kN + tid;
+    if (rest < nv) scalar(rest);
+  } else {
+    for (int k = tid; k < nv; k += kLogitsThreads) scalar(k);
+  }
+
+  unsigned long long key = 0;
+  if constexpr (kRules) {
+    // shared memory: a bitmap of touched elements; times generated, and
+    // kGenerated for being in the history at all; index + 1 of the last bias
+    uint32_t* touched = smem;
+    uint32_t* count = smem + p.size / 32 + 4;
+    uint32_t* bias = count + (kHist ? p.size + 8 : 0);
+    const int vecs = static_cast<int>(bias - smem + (kBias ? p.size + 8 : 0)) / 4;
+    for (int i = tid; i < vecs; i += kLogitsThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    int64_t hbeg = 0, bbeg = 0, end;
+    if constexpr (kHist) row_range(p.r.hist_indptr, row, p.r.n_hist, hbeg, end, p.err);
+    if constexpr (kBias) row_range(p.r.bias_indptr, row, p.r.n_bias, bbeg, end, p.err);
+    const float rep = kHist && p.r.repetition != nullptr ? p.r.repetition[row] : 1.0f;
+    const float freq = kHist && p.r.frequency != nullptr ? p.r.frequency[row] : 0.0f;
+    const float pres = kHist && p.r.presence != nullptr ? p.r.presence[row] : 0.0f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the lists are sorted
+    const int64_t bucket = static_cast<int64_t>(row) * (kBuckets + 1) + (chunk >> p.bucket_shift);
+    const uint32_t* hist_list = nullptr;
+    const uint2* bias_list = nullptr;
+    int n_hist = 0, n_bias = 0;
+    if constexpr (kHist) {
+      const int from = p.sorted.hist_starts[bucket];
+      n_hist = p.sorted.hist_starts[bucket + 1] - from;
+      hist_list = p.sorted.hist + hbeg + from;
+    }
+    if constexpr (kBias) {
+      const int from = p.sorted.bias_starts[bucket];
+      n_bias = p.sorted.bias_starts[bucket + 1] - from;
+      bias_list = p.sorted.bias + bbeg + from;
+    }
+    __syncthreads();  // the tables, and the first pass's stores
+    for (int i = tid; i < n_hist; i += kLogitsThreads) {
+      const uint32_t t = hist_list[i], k = (t & ~kGenerated) - static_cast<uint32_t>(v0);
+      if (k >= static_cast<uint32_t>(nv)) continue;  // another chunk of the bucket
+      if (!(count[k] & kGenerated)) atomicOr(&count[k], kGenerated);
+      if (t & kGenerated) atomicAdd(&count[k], 1u);
+    }
+    for (int i = tid; i < n_bias; i += kLogitsThreads) {
+      const uint32_t k = bias_list[i].x - static_cast<uint32_t>(v0);
+      if (k < static_cast<uint32_t>(nv)) atomicMax(&bias[k], bias_list[i].y + 1u);
+    }
+    __syncthreads();
+    // The first entry to take a token's counts out of the tables applies them.
+    auto apply = [&](uint32_t k, uint32_t in_hist, uint32_t in_bias) {
+      atomicOr(&touched[k >> 5], 1u << (k & 31));
+      if (!allowed(k)) return;
+      float y = ld_logit(in + k);
+      if (in_hist != 0) {
+        const uint32_t n = in_hist & ~kGenerated;
+        y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+        y = __fsub_rn(y, __fmul_rn(freq, static_cast<float>(n)));
+        if (n != 0) y = __fsub_rn(y, pres);
+      }
+      if (in_bias != 0) y = __fadd_rn(y, p.r.bias_values[bbeg + in_bias - 1]);
+      out[k] = y;
+      key = max(key, arg_key(y, v0 + static_cast<int>(k)));
+    };
+    for (int i = tid; i < n_hist; i += kLogitsThreads) {
+      const uint32_t k = (hist_list[i] & ~kGenerated) - static_cast<uint32_t>(v0);
+      if (k >= static_cast<uint32_t>(nv) || count[k] == 0) continue;
+      const uint32_t c = atomicExch(&count[k], 0u);
+      if (c != 0) apply(k, c, kBias ? atomicExch(&bias[k], 0u) : 0u);
+    }
+    if (kHist && kBias) __syncthreads();
+    for (int i = tid; i < n_bias; i += kLogitsThreads) {
+      const uint32_t k = bias_list[i].x - static_cast<uint32_t>(v0);
+      if (k >= static_cast<uint32_t>(nv)) continue;
+      const uint32_t b = atomicExch(&bias[k], 0u);
+      if (b != 0) apply(k, 0u, b);
+    }
+    __syncthreads();
+    auto is_touched = [&](int k) { return (touched[k >> 5] >> (k & 31) & 1u) != 0; };
+    if (p.tokens != nullptr && best > -INFINITY && is_touched(best_k)) {
+      // this thread's maximum is a touched element: look for another (untouched
+      // elements of `out` are final)
+      best = -INFINITY;
+      auto again = [&](int k) {
+        const float y = out[k];
+        if (y > best && !is_touched(k)) best = y, best_k = k;
+      };
+      if (vec) {
+        if (tid < body) again(tid);
+        for (int i = tid; i < nvec; i += kLogitsThreads)
+          for (int e = 0; e < kN; ++e) again(body + i * kN + e);
+        if (body + nvec * kN + tid < nv) again(body + nvec * kN + tid);
+      } else {
+        for (int k = tid; k < nv; k += kLogitsThreads) again(k);
+      }
+    }
   }
   if (p.tokens == nullptr) return;
-  unsigned long long key = arg_key(best, best_v);
+  key = max(key, arg_key(best, v0 + best_k));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
   __shared__ unsigned long long wkey[kLogitsThreads / 32];
@@ -277,12 +402,25 @@ __global__ void __launch_bounds__(kLogitsThreads) process_logits_kernel(const Lo
 #pragma unroll
   for (int w = 1; w < kLogitsThreads / 32; ++w) key = max(key, wkey[w]);
   atomicMax(&p.keys[row], key);
-  __threadfence();
-  if (atomicAdd(&p.keys[p.n_rows + row], 1ull) != static_cast<unsigned long long>(p.chunks - 1)) return;
-  __threadfence();
+  unsigned long long before;  // release: the maximum above; acquire: the other chunks'
+  asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(before) : "l"(&p.keys[p.n_rows + row]) : "memory");
+  if (before != static_cast<unsigned long long>(p.chunks - 1)) return;
   key = atomicExch(&p.keys[row], 0ull);
   p.keys[p.n_rows + row] = 0ull;
   p.tokens[row] = key == 0 ? 0 : static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
+}
+
+using LogitsKernel = void (*)(const LogitsParams);
+
+template <typename T>
+LogitsKernel logits_kernel(bool hist, bool biased) {
+  if (hist) return biased ? process_logits_kernel<T, true, true> : process_logits_kernel<T, true, false>;
+  return biased ? process_logits_kernel<T, false, true> : process_logits_kernel<T, false, false>;
+}
+
+// Shared memory of a chunk of `size` elements, bytes.
+constexpr int logits_smem(int size, bool hist, bool biased) {
+  return hist || biased ? (size / 32 + 4 + (static_cast<int>(hist) + static_cast<int>(biased)) * (size + 8)) * 4 : 0;
 }
 
 }  // namespace
@@ -294,10 +432,17 @@ size_t mtn_process_logits_workspace_bytes(int64_t n_rows) {
   return n_rows <= 0 ? 0 : static_cast<size_t>(n_rows) * 16;
 }
 
+size_t mtn_process_logits_scratch_bytes(int64_t n_rows, int64_t n_hist, int64_t n_bias) {
+  if (n_rows <= 0 || n_hist < 0 || n_bias < 0 || n_hist + n_bias == 0) return 0;
+  // sorted biases and history, and where each row's buckets begin in both
+  return static_cast<size_t>(n_bias) * 8 + static_cast<size_t>(n_hist) * 4 +
+         static_cast<size_t>(n_rows) * (mtn::kBuckets + 1) * 8;
+}
+
 int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, int64_t n_rows, int64_t vocab,
                        const mtn_logits_rules* rules, float* out, int64_t out_stride, int32_t* tokens, void* workspace,
-                       size_t workspace_bytes, void* stream) {
-  MTN_CHECK_ARG(n_rows >= 0 && n_rows <= INT32_MAX && vocab > 0 && vocab <= INT32_MAX, "mtn_process_logits: bad sizes");
+                       size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
+  MTN_CHECK_ARG(n_rows >= 0 && n_rows <= INT32_MAX && vocab > 0 && vocab <= INT32_MAX - 65536, "mtn_process_logits: bad sizes");
   MTN_CHECK_ARG(dtype == MTN_DTYPE_BF16 || dtype == MTN_DTYPE_F32, "mtn_process_logits: bad dtype");
   if (n_rows == 0) return MTN_OK;
   MTN_CHECK_ARG(logits && rules && out, "mtn_process_logits: null pointer");
@@ -323,25 +468,60 @@ int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, in
   MTN_CHECK_ARG(tokens == nullptr || (workspace != nullptr && workspace_bytes >= need &&
                                       (reinterpret_cast<uintptr_t>(workspace) & 7) == 0),
                 "mtn_process_logits: tokens need an 8-byte aligned workspace of %zu bytes", need);
-  // Few rows: small chunks, so that every SM has some.
-  int chunk = mtn::kChunkLarge;
-  if (n_rows * ((vocab + chunk - 1) / chunk) < 2 * mtn::sm_count()) chunk = mtn::kChunkSmall;
-  const int64_t chunks = (vocab + chunk - 1) / chunk;
+  const int64_t n_hist = r.hist_indptr != nullptr ? r.n_hist : 0, n_bias = r.bias_indptr != nullptr ? r.n_bias : 0;
+  const bool ruled = n_hist + n_bias > 0;
+  const size_t lists = mtn_process_logits_scratch_bytes(n_rows, n_hist, n_bias);
+  MTN_CHECK_ARG(!ruled || (scratch != nullptr && scratch_bytes >= lists && (reinterpret_cast<uintptr_t>(scratch) & 7) == 0),
+                "mtn_process_logits: a history or biases need an 8-byte aligned scratch of %zu bytes", lists);
+  // The chunk whose waves of resident CTAs have the fewest elements to pass,
+  // a CTA's fixed part counted as kChunkFixed of them.
+  int size = 0;
+  int64_t chunks = 0, best = INT64_MAX;
+  const bool hist = n_hist > 0, biased = n_bias > 0;
+  for (int sz = mtn::kChunkStep; sz <= (ruled ? mtn::kChunkMaxRuled : mtn::kChunkMax); sz += mtn::kChunkStep) {
+    const int64_t c = (vocab + sz - 1) / sz;
+    const int fit = ruled ? 227 * 1024 / (mtn::logits_smem(sz, hist, biased) + 1024) : mtn::kLogitsResident;
+    const int64_t slots = static_cast<int64_t>(mtn::sm_count()) * std::min(fit, mtn::kLogitsResident);
+    const int64_t cost = (n_rows * c + slots - 1) / slots * (sz + mtn::kChunkFixed);
+    if (cost < best) {
+      best = cost;
+      size = sz;
+      chunks = c;
+    }
+  }
   MTN_CHECK_ARG(chunks * n_rows <= INT32_MAX, "mtn_process_logits: batch too large");
-  mtn::LogitsParams p{logits, row_stride, vocab, r, out, out_stride, tokens,
-                      static_cast<unsigned long long*>(workspace), n_rows, static_cast<int>(chunks), chunk,
-                      mtn::device_error_ptr()};
-  const size_t table = static_cast<size_t>(chunk + 8) * 4;
-  size_t smem = 0;
-  if (r.hist_indptr != nullptr || r.bias_indptr != nullptr) smem += (static_cast<size_t>(chunk) / 32 + 2 + 3) / 4 * 16;
-  if (r.hist_indptr != nullptr) smem += table;
-  if (r.bias_indptr != nullptr) smem += table;
-  auto kern = dtype == MTN_DTYPE_BF16 ? mtn::process_logits_kernel<__nv_bfloat16> : mtn::process_logits_kernel<float>;
-  if (smem > 48 * 1024)
-    MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
-                 "mtn_process_logits");
-  kern<<<static_cast<unsigned>(chunks * n_rows), mtn::kLogitsThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
-  return mtn::check_launch("process_logits_kernel");
+  mtn::SortedRules l{};
+  if (ruled) {
+    l.bias = static_cast<uint2*>(scratch);
+    l.hist = reinterpret_cast<uint32_t*>(l.bias + n_bias);
+    l.hist_starts = reinterpret_cast<int32_t*>(l.hist + n_hist);
+    l.bias_starts = l.hist_starts + n_rows * (mtn::kBuckets + 1);
+  }
+  int bucket_shift = 0;
+  while ((chunks - 1) >> bucket_shift >= mtn::kBuckets) ++bucket_shift;
+  const bool bf16 = dtype == MTN_DTYPE_BF16;
+  mtn::LogitsParams p{logits, row_stride, vocab, r, l, out, out_stride, tokens, static_cast<unsigned long long*>(workspace),
+                      n_rows, static_cast<int>(chunks), size, bf16 ? 2 : 4, bucket_shift, mtn::device_error_ptr()};
+  if (!hist) p.r.hist_indptr = nullptr;
+  if (!biased) p.r.bias_indptr = nullptr;
+  auto s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = static_cast<unsigned>(chunks * n_rows);
+  const mtn::LogitsKernel kern =
+      bf16 ? mtn::logits_kernel<__nv_bfloat16>(hist, biased) : mtn::logits_kernel<float>(hist, biased);
+  if (!ruled) {
+    kern<<<grid, mtn::kLogitsThreads, 0, s>>>(p);
+    return mtn::check_launch("process_logits_kernel");
+  }
+  mtn::sort_rules_kernel<<<static_cast<unsigned>(n_rows), mtn::kSortThreads, 0, s>>>(p);
+  const int st = mtn::check_launch("sort_rules_kernel");
+  if (st != MTN_OK) return st;
+  const int smem = mtn::logits_smem(size, hist, biased);
+  MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    mtn::logits_smem(mtn::kChunkMaxRuled, true, true)),
+               "mtn_process_logits");
+  MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared),
+               "mtn_process_logits");
+  return mtn::launch_pdl(kern, dim3(grid), dim3(mtn::kLogitsThreads), smem, s, "process_logits_kernel", p);
 }
 
 }  // extern "C"

@@ -411,6 +411,7 @@ class LogitsRules:
             0 if mask is None else (mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]),
             0 if mask is None else mask.shape[0], _ptr(mask_rows))
         self._ref = C.byref(self.struct)
+        self.entries = (n(hist_tokens), n(bias_tokens))
 
 
 def logits_workspace(n_rows: int, device) -> torch.Tensor:
@@ -453,10 +454,16 @@ def process_logits(logits: torch.Tensor, rules: LogitsRules, out: torch.Tensor |
     for t in (out, tokens, workspace, rules):
         if t is not None and t.device not in (None, logits.device):
             raise ValueError(f"tensors on {t.device} and {logits.device}")
+    scratch = None
+    if n and any(rules.entries):
+        with torch.cuda.stream(stream):  # the memory belongs to the launch's stream
+            scratch = torch.empty(L.lib().mtn_process_logits_scratch_bytes(n, *rules.entries), dtype=torch.uint8,
+                                  device=logits.device)
     st = (lambda t: t.stride(0) if n > 1 else vocab)
     L.check(L.lib().mtn_process_logits(_ptr(logits), _dtype_code(logits.dtype), st(logits), n, vocab, rules._ref,
                                        _ptr(out), st(out), _ptr(tokens), _ptr(workspace),
-                                       0 if workspace is None else workspace.numel(), _stream(stream)))
+                                       0 if workspace is None else workspace.numel(), _ptr(scratch),
+                                       0 if scratch is None else scratch.numel(), _stream(stream)))
     return out, tokens
 
 

@@ -160,6 +160,30 @@ def test_ties_go_to_the_lowest_index(cuda_device):
     assert tok.tolist() == [9000, 0, 20000]
 
 
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("kind", ["distinct", "repeats"])
+@pytest.mark.parametrize("n", [500, 16384, 16385, 40000])
+def test_long_histories(cuda_device, kind, n):
+    """Histories of many steps of the sorting kernel: all different, and few that repeat."""
+    rng = np.random.default_rng(n)
+    vocab = 150001
+    c = _case(rng, 3, vocab, 50, 40, 2)
+    pick = rng.choice(7, n) * 1000 if kind == "repeats" else rng.permutation(vocab)[:n]
+    c["hist"][1] = pick.astype(np.int32)
+    c["prompt"][1] = len(pick) // 3
+    _check(torch.from_numpy(rng.standard_normal((3, vocab)).astype(np.float32) * 3), c, _rules(c))
+    assert paged.device_error(0) == (0, 0)
+
+
+def test_vocabulary_of_more_chunks_than_buckets(cuda_device):
+    rng = np.random.default_rng(6)
+    vocab = 40_000_003
+    c = _case(rng, 1, vocab, 3000, 100, None)
+    x = torch.randn(1, vocab)
+    x[0, 39_999_999] = 50.0
+    _check(x, c, _rules(c))
+
+
 @pytest.mark.parametrize("off,pad", [(0, 3), (1, 0), (2, 5), (3, 1), (4, 4), (5, 2)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strided_rows(cuda_device, off, pad, dtype):

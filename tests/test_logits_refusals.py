@@ -11,10 +11,10 @@ P = [0x100000 * (i + 1) for i in range(8)]
 
 
 def _call(rules=None, no_rules=False, logits=P[0], dtype=_lib.MTN_DTYPE_F32, stride=100, n=2, vocab=100, out=P[1],
-          out_stride=100, tokens=None, ws=None, ws_bytes=0):
+          out_stride=100, tokens=None, ws=None, ws_bytes=0, scratch=P[5], scratch_bytes=1 << 20):
     r = _lib.LogitsRules(**(rules or {}))
     return _lib.lib().mtn_process_logits(logits, dtype, stride, n, vocab, None if no_rules else C.byref(r), out,
-                                         out_stride, tokens, ws, ws_bytes, None)
+                                         out_stride, tokens, ws, ws_bytes, scratch, scratch_bytes, None)
 
 
 @pytest.mark.parametrize("kw,msg", [
@@ -30,7 +30,11 @@ def _call(rules=None, no_rules=False, logits=P[0], dtype=_lib.MTN_DTYPE_F32, str
     (dict(rules=dict(mask_rows=P[2])), b"without a mask"),
     (dict(tokens=P[3]), b"workspace"), (dict(tokens=P[3], ws=P[4], ws_bytes=31), b"workspace"),
     (dict(tokens=P[3], ws=P[4] + 4, ws_bytes=64), b"aligned"),
-    (dict(n=2 ** 31 - 1, vocab=2 ** 31 - 1, stride=2 ** 31, out_stride=2 ** 31), b"batch too large"),
+    (dict(vocab=2 ** 31 - 1, stride=2 ** 31, out_stride=2 ** 31), b"bad sizes"),
+    (dict(n=2 ** 31 - 1, vocab=2 ** 30, stride=2 ** 31, out_stride=2 ** 31), b"batch too large"),
+    (dict(rules=dict(hist_indptr=P[2], hist_tokens=P[3], n_hist=10), scratch=None), b"aligned scratch"),
+    (dict(rules=dict(hist_indptr=P[2], hist_tokens=P[3], n_hist=10), scratch_bytes=127), b"aligned scratch"),
+    (dict(rules=dict(hist_indptr=P[2], hist_tokens=P[3], n_hist=10), scratch=P[5] + 4), b"aligned scratch"),
 ])
 def test_refuses(kw, msg):
     assert _call(**kw) == _lib.MTN_EINVAL
