@@ -196,8 +196,12 @@ constexpr int kMinUnits = 8;    // row units of a round that the slots of a spli
 constexpr int kJoinSteps = 16;
 constexpr int kSmemMax = 225 * 1024;
 
-constexpr int mv_units(int parts, int nt) { return parts * nt > 1 ? 2 : 1; }          // kR
-constexpr int mv_depth(int parts, int nt) { return mv_units(parts, nt) > 1 ? 2 : 5; }  // kD
+// Row units of a step: one, or two that share their x fragments where those
+// are many, or where the steps of a warp are (kSteps2): 1 x 152064 x 3584 took
+// 55.7 us with one and 51.9 with two, 8 x 3584 x 18944 13.9 and 15.2.
+constexpr int mv_units(int parts, int nt, bool many) { return parts * nt > 1 || many ? 2 : 1; }  // kR
+constexpr int mv_depth(int r) { return r > 1 ? 2 : 5; }                                          // kD
+constexpr int64_t kSteps2 = 32;
 constexpr int mv_stage(int r, int groups) { return r * (1024 + 32 * groups); }         // bytes of a step
 constexpr int mv_slot(int r, int nt) { return 16 * r * 8 * nt; }                       // floats of a slot
 
@@ -208,7 +212,8 @@ struct MvPlan {
   int tile;        // x rows of one pass
   int units_cap;   // row units of one round
   int x_stride;    // elements between staged rows
-  int x_vec;       // x rows allow 16-byte loads
+  int units;       // row units of a step
+  int x_vec;       // x rows allow vector loads
   size_t smem, ring_off, slots_off;
 };
 
@@ -307,32 +312,44 @@ __device__ __forceinline__ void store_out(const W4Params& p, int64_t m, int64_t 
     static_cast<float*>(p.out)[m * p.out_stride + n] = v;
 }
 
-// Eight consecutive elements of an x row; `vec`: 16-byte loads are aligned.
+// Eight consecutive elements of an x row as loaded, zeros beyond k: two words
+// of e4m3, four of bf16, eight of f32.  `vec`: the row allows vector loads.
+struct Raw8 {
+  uint32_t w[8];
+};
+
 template <int kParts>
-__device__ __forceinline__ void load8(const W4Params& p, int64_t at, int64_t k, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load_raw(const W4Params& p, int64_t at, int64_t k, bool vec, Raw8& r) {
   if (vec && k + 8 <= p.k) {
     if constexpr (kParts == 3) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + at);
-      const float4 a = q[0], b = q[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else if (p.x_dtype == MTN_DTYPE_BF16) {
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[2 * i] = bf2_to_f2(w[i]).x, v[2 * i + 1] = bf2_to_f2(w[i]).y;
-    } else {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + at);
+      const uint4 a = q[0], b = q[1];
+      r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w, r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+    } else {  // e4m3; aligned bf16 rows are copied as they are
       const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.x) + at);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        __nv_fp8_e4m3 e;
-        e.__x = static_cast<uint8_t>((i < 4 ? a.x : a.y) >> (8 * (i & 3)));
-        v[i] = static_cast<float>(e);
-      }
+      r.w[0] = a.x, r.w[1] = a.y;
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = k + i < p.k ? ld_any(p.x, at + i, kParts == 3 ? MTN_DTYPE_F32 : p.x_dtype) : 0.0f;
+  for (int i = 0; i < 8; ++i) r.w[i] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (k + i >= p.k) break;
+    if constexpr (kParts == 3)
+      r.w[i] = static_cast<const uint32_t*>(p.x)[at + i];
+    else if (p.x_dtype == MTN_DTYPE_BF16)
+      r.w[i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p.x)[at + i]) << (16 * (i & 1));
+    else
+      r.w[i / 4] |= static_cast<uint32_t>(static_cast<const uint8_t*>(p.x)[at + i]) << (8 * (i & 3));
+  }
+}
+
+// Two e4m3 values of a word's half as bf16x2 (exact).
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w, int half) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * half)), __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  return f2_to_bf2(f.x, f.y);
 }
 
 // Copies x rows m0 .. m0 + mt, k0 .. k0 + len, to shared memory as they are
@@ -349,39 +366,50 @@ __device__ __forceinline__ void copy_rows(const W4Params& p, const MvPlan& plan,
 }
 
 // The same through registers, for every other row: f32 cut into three bf16
-// parts, e4m3 exact in bf16, unaligned rows.  kBatch rows are in flight.
-template <int kParts>
+// parts, e4m3 exact in bf16, unaligned rows.  kBatch rows are in flight;
+// then() runs once, behind the last of this thread's loads.
+template <int kParts, typename F>
 __device__ __forceinline__ void convert_rows(const W4Params& p, const MvPlan& plan, uint16_t* xs, int64_t m0, int mt,
-                                             int64_t k0, int len) {
-  constexpr int kBatch = kParts == 3 ? 2 : 4;
-  for (int e = threadIdx.x * 8; e < len; e += kMvThreads * 8) {
+                                             int64_t k0, int len, F then) {
+  constexpr int kBatch = kParts == 3 ? 4 : 8;
+  const int step = static_cast<int>(blockDim.x) * 8;
+  bool done = false;
+  for (int e = threadIdx.x * 8; e < len; e += step) {
     for (int mb = 0; mb < mt; mb += kBatch) {
-      float v[kBatch][8];
+      Raw8 v[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b)
-        if (mb + b < mt) load8<kParts>(p, (m0 + mb + b) * p.x_stride + k0 + e, k0 + e, plan.x_vec != 0, v[b]);
+        if (mb + b < mt) load_raw<kParts>(p, (m0 + mb + b) * p.x_stride + k0 + e, k0 + e, plan.x_vec != 0, v[b]);
+      if (e + step >= len && mb + kBatch >= mt) {
+        then();
+        done = true;
+      }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         if (mb + b >= mt) continue;
         uint16_t* dst = xs + (mb + b) * plan.x_stride + e;
+        const uint32_t* w = v[b].w;
         if constexpr (kParts == 1) {
-          *reinterpret_cast<uint4*>(dst) = make_uint4(f2_to_bf2(v[b][0], v[b][1]), f2_to_bf2(v[b][2], v[b][3]),
-                                                      f2_to_bf2(v[b][4], v[b][5]), f2_to_bf2(v[b][6], v[b][7]));
+          *reinterpret_cast<uint4*>(dst) =
+              p.x_dtype == MTN_DTYPE_BF16
+                  ? make_uint4(w[0], w[1], w[2], w[3])
+                  : make_uint4(e4m3_pair(w[0], 0), e4m3_pair(w[0], 1), e4m3_pair(w[1], 0), e4m3_pair(w[1], 1));
         } else {
           uint16_t h[8][3];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) split3(v[b][j], h[j]);
+          for (int j = 0; j < 8; ++j) split3(__uint_as_float(w[j]), h[j]);
 #pragma unroll
           for (int q = 0; q < 3; ++q) {
-            uint32_t w[4];
+            uint32_t o[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = h[2 * j][q] | static_cast<uint32_t>(h[2 * j + 1][q]) << 16;
-            *reinterpret_cast<uint4*>(dst + q * plan.tile * plan.x_stride) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 4; ++j) o[j] = h[2 * j][q] | static_cast<uint32_t>(h[2 * j + 1][q]) << 16;
+            *reinterpret_cast<uint4*>(dst + q * plan.tile * plan.x_stride) = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
       }
     }
   }
+  if (!done) then();
 }
 
 // kParts: bf16 parts of an x value (1, or 3 for f32).  kNT: 8-row tiles of
@@ -451,22 +479,38 @@ __global__ void __launch_bounds__(kMvThreads, 1) w4_matvec_kernel(const W4Params
         seek();
       }
     };
-    // x before the weights: behind them it would wait for all their bytes
-    if (u0 == cu0) {
-      if (direct) copy_rows(p, plan, smem_u32(xs), m0, mt, k0, L * kKPad);
-      cp_async_commit();
-    }
-    seek();
+    auto fill = [&]() {
+      seek();
 #pragma unroll
-    for (int d = 0; d < kD; ++d) {
-      if (d < n_items) load(ring + d * kStage);
-      cp_async_commit();
-    }
-
+      for (int d = 0; d < kD; ++d) {
+        if (d < n_items) load(ring + d * kStage);
+        cp_async_commit();
+      }
+    };
     if (u0 == cu0) {
-      if (!direct) convert_rows<kParts>(p, plan, xs, m0, mt, k0, L * kKPad);
-      cp_async_wait<kD>();  // the copied rows, not the weights behind them
+      // What the kernel before this one does not write may start early: the
+      // weights on their way into L2.
+      seek();
+      for (int d = 0; d < min(min(kD, n_items), L - ls); ++d)
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+          const uint4* w = wp[r] + d * 64;
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(w));
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(w + 32));
+        }
+      pdl_enter();
+      // x before the weights: behind them it would wait for all their bytes
+      if (direct) {
+        copy_rows(p, plan, smem_u32(xs), m0, mt, k0, L * kKPad);
+        cp_async_commit();
+        fill();
+      } else {
+        convert_rows<kParts>(p, plan, xs, m0, mt, k0, L * kKPad, fill);
+      }
+      if (direct) cp_async_wait<kD>();  // the copied rows, not the weights behind them
       __syncthreads();
+    } else {
+      fill();
     }
 
     float acc[kR][kNT][4] = {};
@@ -624,14 +668,20 @@ __global__ void __launch_bounds__(kMvThreads, 1) w4_matvec_kernel(const W4Params
 
 using MvKernel = void (*)(const W4Params, const MvPlan);
 
-template <int kParts, int kNT>
+template <int kParts, int kNT, int kR>
 MvKernel mv_kernel(int group) {
-  constexpr int kR = mv_units(kParts, kNT), kD = mv_depth(kParts, kNT);
+  constexpr int kD = mv_depth(kR);
   switch (group) {
     case 32: return w4_matvec_kernel<kParts, kNT, kR, 4, kD>;
     case 64: return w4_matvec_kernel<kParts, kNT, kR, 2, kD>;
     default: return w4_matvec_kernel<kParts, kNT, kR, 1, kD>;
   }
+}
+
+MvKernel mv_kernel(int parts, int nt, int r, int group) {
+  if (parts == 3) return nt > 1 ? mv_kernel<3, 2, 2>(group) : mv_kernel<3, 1, 2>(group);
+  if (nt > 1) return mv_kernel<1, 2, 2>(group);
+  return r > 1 ? mv_kernel<1, 1, 2>(group) : mv_kernel<1, 1, 1>(group);
 }
 
 // Clusters of `size` CTAs that the device holds at once (one CTA per SM).
@@ -654,7 +704,7 @@ int max_clusters(int size) {
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      auto kern = mv_kernel<1, 1>(128);
+      const MvKernel kern = mv_kernel(1, 1, 1, 128);
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax)) !=
               cudaSuccess ||
           cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
@@ -677,10 +727,11 @@ MvPlan mv_plan(int64_t m, int64_t n, int64_t k, int group, int parts) {
   pl.tile = static_cast<int>(std::min<int64_t>(m, 16));
   int nt, r;
   size_t ring, slot;
+  const bool many = row_units(n) * ksteps >= kSteps2 * kMvWarps * sm_count();
   auto sizes = [&]() {
     nt = pl.tile > 8 ? 2 : 1;
-    r = mv_units(parts, nt);
-    ring = static_cast<size_t>(kMvWarps) * mv_depth(parts, nt) * mv_stage(r, kKPad / group);
+    r = mv_units(parts, nt, many);
+    ring = static_cast<size_t>(kMvWarps) * mv_depth(r) * mv_stage(r, kKPad / group);
     slot = static_cast<size_t>(mv_slot(r, nt)) * 4;
   };
   auto x_bytes = [&](int s) {
@@ -715,6 +766,7 @@ MvPlan mv_plan(int64_t m, int64_t n, int64_t k, int group, int parts) {
       pl.units_cap = static_cast<int>((per + rounds - 1) / rounds);
     }
   }
+  pl.units = r;
   pl.x_stride = (ksteps + pl.cluster - 1) / pl.cluster * kKPad + kXPad;
   pl.ring_off = x_bytes(pl.cluster);
   pl.slots_off = pl.ring_off + ring;
@@ -813,9 +865,7 @@ int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float*
   const int elem = x_dtype == MTN_DTYPE_F32 ? 4 : x_dtype == MTN_DTYPE_BF16 ? 2 : 1;
   const int64_t vec = elem == 1 ? 8 : 16;  // bytes of one vector load
   plan.x_vec = reinterpret_cast<uintptr_t>(x) % vec == 0 && (n_rows == 1 || x_stride * elem % vec == 0);
-  const bool two = plan.tile > 8;
-  const mtn::MvKernel kern = parts == 1 ? (two ? mtn::mv_kernel<1, 2>(group) : mtn::mv_kernel<1, 1>(group))
-                                        : (two ? mtn::mv_kernel<3, 2>(group) : mtn::mv_kernel<3, 1>(group));
+  const mtn::MvKernel kern = mtn::mv_kernel(parts, plan.tile > 8 ? 2 : 1, plan.units, group);
   MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(mtn::kSmemMax)),
                "mtn_w4_matvec");
   cudaLaunchConfig_t cfg = {};
@@ -824,12 +874,14 @@ int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float*
   cfg.blockDim = dim3(mtn::kMvThreads);
   cfg.dynamicSmemBytes = plan.smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(plan.cluster);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   MTN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, plan), "w4_matvec_kernel");
   return mtn::check_launch("w4_matvec_kernel");
 }
