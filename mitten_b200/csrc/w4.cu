@@ -352,16 +352,32 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w, int half) {
   return f2_to_bf2(f.x, f.y);
 }
 
+// A thread's part of staged rows of `len` elements: the vector of 8 at `first`
+// of every `rows`-th row from `row` on (rows longer than the CTA's vectors:
+// every row, and the vectors kMvThreads apart).
+struct RowSplit {
+  int first, row, rows;
+  __device__ __forceinline__ explicit RowSplit(int len) {
+    const int per = len / 8, tid = static_cast<int>(threadIdx.x);
+    rows = per > 0 && per < kMvThreads ? kMvThreads / per : 1;
+    row = rows > 1 ? tid / per : 0;
+    first = (tid - row * per) * 8;
+    if (row >= rows) first = len;  // the threads left over
+  }
+};
+
 // Copies x rows m0 .. m0 + mt, k0 .. k0 + len, to shared memory as they are
 // (aligned bf16 rows), zeros beyond k; asynchronous.
 __device__ __forceinline__ void copy_rows(const W4Params& p, const MvPlan& plan, uint32_t xs, int64_t m0, int mt,
                                           int64_t k0, int len) {
   const uint16_t* x = static_cast<const uint16_t*>(p.x) + m0 * p.x_stride + k0;
-  for (int v = threadIdx.x * 8; v < len; v += kMvThreads * 8) {
+  const RowSplit t(len);
+  for (int v = t.first; v < len; v += kMvThreads * 8) {
     const int64_t left = (p.k - k0 - v) * 2;
     const uint32_t bytes = left >= 16 ? 16u : left > 0 ? static_cast<uint32_t>(left) : 0u;
     const uint16_t* src = bytes > 0 ? x + v : x;
-    for (int m = 0; m < mt; ++m) cp_async16_fill(xs + (m * plan.x_stride + v) * 2, src + m * p.x_stride, bytes);
+    for (int m = t.row; m < mt; m += t.rows)
+      cp_async16_fill(xs + (m * plan.x_stride + v) * 2, src + m * p.x_stride, bytes);
   }
 }
 
@@ -372,22 +388,24 @@ template <int kParts, typename F>
 __device__ __forceinline__ void convert_rows(const W4Params& p, const MvPlan& plan, uint16_t* xs, int64_t m0, int mt,
                                              int64_t k0, int len, F then) {
   constexpr int kBatch = kParts == 3 ? 4 : 8;
-  const int step = static_cast<int>(blockDim.x) * 8;
+  const int step = kMvThreads * 8;
+  const RowSplit t(len);
   bool done = false;
-  for (int e = threadIdx.x * 8; e < len; e += step) {
-    for (int mb = 0; mb < mt; mb += kBatch) {
+  for (int e = t.first; e < len; e += step) {
+    for (int mb = t.row; mb < mt; mb += kBatch * t.rows) {
       Raw8 v[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b)
-        if (mb + b < mt) load_raw<kParts>(p, (m0 + mb + b) * p.x_stride + k0 + e, k0 + e, plan.x_vec != 0, v[b]);
-      if (e + step >= len && mb + kBatch >= mt) {
+        if (mb + b * t.rows < mt)
+          load_raw<kParts>(p, (m0 + mb + b * t.rows) * p.x_stride + k0 + e, k0 + e, plan.x_vec != 0, v[b]);
+      if (e + step >= len && mb + kBatch * t.rows >= mt) {
         then();
         done = true;
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        if (mb + b >= mt) continue;
-        uint16_t* dst = xs + (mb + b) * plan.x_stride + e;
+        if (mb + b * t.rows >= mt) continue;
+        uint16_t* dst = xs + (mb + b * t.rows) * plan.x_stride + e;
         const uint32_t* w = v[b].w;
         if constexpr (kParts == 1) {
           *reinterpret_cast<uint4*>(dst) =
@@ -617,22 +635,19 @@ __global__ void __launch_bounds__(kMvThreads, 1) w4_matvec_kernel(const W4Params
       // those of the cluster's CTAs.
       float* part = reinterpret_cast<float*>(smem + plan.ring_off);
       __syncthreads();
-      for (int q = warp; q < nu; q += kMvWarps) {
-        int wa = 0, wb = -1;  // first and last warp with a step of unit q
-        if (L > 0) {
-          wa = ((q * L + 1) * kMvWarps - 1) / total;
-          wb = ((q + 1) * L * kMvWarps - 1) / total;
-        }
-        for (int i = lane; i < mt * kUnitRows; i += 32) {
-          float v = 0.0f;
+      const int per_unit = mt * kUnitRows;
+      for (int i = tid; i < nu * per_unit; i += kMvThreads) {
+        const int q = i / per_unit, off = i - q * per_unit;
+        float v = 0.0f;
+        if (L > 0) {  // first to last warp with a step of unit q
+          const int wa = ((q * L + 1) * kMvWarps - 1) / total, wb = ((q + 1) * L * kMvWarps - 1) / total;
           for (int w = wa; w <= wb; ++w)
-            if (w * total / kMvWarps != (w + 1) * total / kMvWarps) v += slots[(q + w) * kSlot + i];
-          part[q * kSlot + i] = v;
+            if (w * total / kMvWarps != (w + 1) * total / kMvWarps) v += slots[(q + w) * kSlot + off];
         }
+        part[q * kSlot + off] = v;
       }
       cluster_sync();
       const uint32_t part_at = smem_u32(part);
-      const int per_unit = mt * kUnitRows;
       for (int i = rank * kMvThreads + tid; i < nu * per_unit; i += S * kMvThreads) {
         const int q = i / per_unit, off = i - q * per_unit;
         float v[8];
