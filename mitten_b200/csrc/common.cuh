@@ -69,6 +69,11 @@ int validate_layout(const mtn_kv_layout* pool, int layer, const char* who);
 // SM count of the current device (cached per device).
 int sm_count();
 
+// Lets `kernel` have up to `bytes` of dynamic shared memory on the current
+// device and prefers shared memory over L1 for it; a driver call only the
+// first time for a kernel and device (`bytes` is one value per kernel).
+cudaError_t allow_smem(const void* kernel, int bytes);
+
 // Internal forms of mtn_paged_prefill / mtn_paged_decode_with_plan for the
 // shared-prefix decode: `lse` (or null) receives each (row, query head)'s
 // log2-domain log-sum-exp; `noncausal` lets every prefill query see every

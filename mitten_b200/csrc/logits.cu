@@ -516,10 +516,7 @@ int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, in
   const int st = mtn::check_launch("sort_rules_kernel");
   if (st != MTN_OK) return st;
   const int smem = mtn::logits_smem(size, hist, biased);
-  MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    mtn::logits_smem(mtn::kChunkMaxRuled, true, true)),
-               "mtn_process_logits");
-  MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared),
+  MTN_CUDA_TRY(mtn::allow_smem(reinterpret_cast<const void*>(kern), mtn::logits_smem(mtn::kChunkMaxRuled, true, true)),
                "mtn_process_logits");
   return mtn::launch_pdl(kern, dim3(grid), dim3(mtn::kLogitsThreads), smem, s, "process_logits_kernel", p);
 }

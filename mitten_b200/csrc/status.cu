@@ -1,5 +1,6 @@
 // Status codes, the thread-local last-error string, the per-device error
 // word kernels write instead of trapping, and small C-ABI utilities.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -49,6 +50,34 @@ int sm_count() {
     cached[dev] = n;
   }
   return cached[dev];
+}
+
+cudaError_t allow_smem(const void* kernel, int bytes) {
+  // (kernel, device) pairs already set; entries are only ever added
+  constexpr int kMax = 256;
+  static std::atomic<const void*> kernels[kMax];
+  static std::atomic<int> devices[kMax];
+  static std::atomic<int> count{0};
+  static std::mutex mu;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const int n = count.load(std::memory_order_acquire);
+  for (int i = 0; i < n; ++i)
+    if (kernels[i].load(std::memory_order_relaxed) == kernel && devices[i].load(std::memory_order_relaxed) == dev)
+      return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  const int at = count.load(std::memory_order_relaxed);
+  if (at < kMax) {
+    kernels[at].store(kernel, std::memory_order_relaxed);
+    devices[at].store(dev, std::memory_order_relaxed);
+    count.store(at + 1, std::memory_order_release);
+  }
+  return cudaSuccess;
 }
 
 int* device_error_ptr() {

@@ -720,8 +720,7 @@ int max_clusters(int size) {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       const MvKernel kern = mv_kernel(1, 1, 1, 128);
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMax)) !=
-              cudaSuccess ||
+      if (allow_smem(reinterpret_cast<const void*>(kern), kSmemMax) != cudaSuccess ||
           cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
         cudaGetLastError();
         n = std::max(1, 128 / size);
@@ -881,8 +880,7 @@ int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float*
   const int64_t vec = elem == 1 ? 8 : 16;  // bytes of one vector load
   plan.x_vec = reinterpret_cast<uintptr_t>(x) % vec == 0 && (n_rows == 1 || x_stride * elem % vec == 0);
   const mtn::MvKernel kern = mtn::mv_kernel(parts, plan.tile > 8 ? 2 : 1, plan.units, group);
-  MTN_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(mtn::kSmemMax)),
-               "mtn_w4_matvec");
+  MTN_CUDA_TRY(mtn::allow_smem(reinterpret_cast<const void*>(kern), mtn::kSmemMax), "mtn_w4_matvec");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(plan.clusters * plan.cluster),
                      static_cast<unsigned>((n_rows + plan.tile - 1) / plan.tile));

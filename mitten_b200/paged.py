@@ -356,6 +356,10 @@ def sample_rows(logits: torch.Tensor, temperatures: torch.Tensor, out: torch.Ten
     return out
 
 
+_LOGIT_TYPES = {torch.float32: L.MTN_DTYPE_F32, torch.bfloat16: L.MTN_DTYPE_BF16}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 class LogitsRules:
     """What the rows of a batch ask of their logits (mtn_logits_rules): CUDA tensors on one device, each group
     optional.
@@ -412,6 +416,15 @@ class LogitsRules:
             0 if mask is None else mask.shape[0], _ptr(mask_rows))
         self._ref = C.byref(self.struct)
         self.entries = (n(hist_tokens), n(bias_tokens))
+        self.device_index = None if self.device is None else self.device.index
+        self._scratch = (0, 0)  # (rows, bytes) last asked for
+
+
+    def scratch_bytes(self, n_rows: int) -> int:
+        """Bytes of scratch that mtn_process_logits needs for these lists."""
+        if self._scratch[0] != n_rows:
+            self._scratch = (n_rows, int(L.lib().mtn_process_logits_scratch_bytes(n_rows, *self.entries)))
+        return self._scratch[1]
 
 
 def logits_workspace(n_rows: int, device) -> torch.Tensor:
@@ -428,42 +441,59 @@ def process_logits(logits: torch.Tensor, rules: LogitsRules, out: torch.Tensor |
     `out` may be the f32 logits themselves.  With `tokens` (int32 [rows]) or `greedy` the first strict maximum of
     every processed row comes back too, as argmax_rows gives it; that needs `workspace` (logits_workspace; a fresh
     one is made when none is given)."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (
-            logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError("logits must be a [rows, vocab] f32 or bf16 tensor of unit-stride rows")
-    if logits.is_cuda and logits.device.index != torch.cuda.current_device():
-        with torch.cuda.device(logits.device):
+    code = _LOGIT_TYPES.get(logits.dtype)
+    if code is None or logits.dim() != 2:
+        raise ValueError("logits must be a [rows, vocab] f32 or bf16 tensor")
+    if not logits.is_cuda:
+        raise ValueError("expected a CUDA tensor (there is no CPU implementation)")
+    dev = logits.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
             return process_logits(logits, rules, out, tokens, greedy, workspace, stream)
-    n, vocab = logits.shape
-    if rules.rows not in (None, n):
+    shape = logits.shape
+    n, vocab = shape
+    row, unit = logits.stride()
+    if unit != 1 and vocab > 1:
+        raise ValueError("logits must have unit-stride rows")
+    if rules.rows is not None and rules.rows != n:
         raise ValueError(f"rules for {rules.rows} rows, logits of {n}")
     if rules.masks is not None and (rules.mask_words * 32 < vocab or rules.masks[1] and rules.masks[0] < n):
         raise ValueError("the mask is smaller than the logits")
+    if rules.device_index is not None and rules.device_index != dev:
+        raise ValueError(f"the rules are on cuda:{rules.device_index}, the logits on cuda:{dev}")
     if out is None:
-        out = torch.empty((n, vocab), dtype=torch.float32, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != torch.float32 or (out.stride(1) != 1 and vocab > 1):
-        raise ValueError("out must be an f32 tensor of the logits' shape with unit-stride rows")
+        out = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    out_row, unit = out.stride() if out.dim() == 2 else (0, 0)
+    if out.shape != shape or out.dtype != torch.float32 or (unit != 1 and vocab > 1) or out.get_device() != dev:
+        raise ValueError("out must be an f32 tensor of the logits' shape and device with unit-stride rows")
+    if n <= 1:
+        row = out_row = vocab  # a single row's stride says nothing
+    ws = nws = tp = None
     if tokens is None and greedy:
         tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
     if tokens is not None:
-        if tokens.shape != (n,):
-            raise ValueError("one token per row")
-        _i32(tokens)
+        if tokens.shape != (n,) or tokens.dtype != torch.int32 or not tokens.is_contiguous() or tokens.get_device() != dev:
+            raise ValueError("tokens must be a contiguous int32 tensor of one per row on the logits' device")
+        tp = tokens.data_ptr()
         if workspace is None:
             workspace = logits_workspace(n, logits.device)
-    for t in (out, tokens, workspace, rules):
-        if t is not None and t.device not in (None, logits.device):
-            raise ValueError(f"tensors on {t.device} and {logits.device}")
-    scratch = None
-    if n and any(rules.entries):
-        with torch.cuda.stream(stream):  # the memory belongs to the launch's stream
-            scratch = torch.empty(L.lib().mtn_process_logits_scratch_bytes(n, *rules.entries), dtype=torch.uint8,
-                                  device=logits.device)
-    st = (lambda t: t.stride(0) if n > 1 else vocab)
-    L.check(L.lib().mtn_process_logits(_ptr(logits), _dtype_code(logits.dtype), st(logits), n, vocab, rules._ref,
-                                       _ptr(out), st(out), _ptr(tokens), _ptr(workspace),
-                                       0 if workspace is None else workspace.numel(), _ptr(scratch),
-                                       0 if scratch is None else scratch.numel(), _stream(stream)))
+        elif workspace.get_device() != dev:
+            raise ValueError("the workspace is on another device")
+        ws, nws = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if n == 0:
+        return out, tokens
+    scratch, nscratch = None, rules.scratch_bytes(n)
+    if nscratch:
+        if stream is None:
+            scratch = torch.empty(nscratch, dtype=torch.uint8, device=logits.device)
+        else:
+            with torch.cuda.stream(stream):  # the memory belongs to the launch's stream
+                scratch = torch.empty(nscratch, dtype=torch.uint8, device=logits.device)
+    st = L.lib().mtn_process_logits(logits.data_ptr(), code, row, n, vocab, rules._ref, out.data_ptr(), out_row, tp, ws,
+                                    nws or 0, None if scratch is None else scratch.data_ptr(), nscratch,
+                                    torch._C._cuda_getCurrentRawStream(dev) if stream is None else int(stream.cuda_stream))
+    if st:
+        L.check(st)
     return out, tokens
 
 
