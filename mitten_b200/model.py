@@ -24,16 +24,23 @@ The same class is the attention call site the Gemma crate lacks
 layer at Gemma-2B shapes (MQA, head_dim 256, GeGLU MLP, theta 1e4) without
 the Qwen gate, q/k norms or phantom row (Gemma's caches start empty,
 model.rs:96-105).
+
+With `w4_group` the projections, the MLP and the LM head keep their weights
+in 4 bits (mitten_b200.dense): a decode step runs mtn_add_rms_norm and
+mtn_w4_matvec in place of torch's norms and matrix products, with q/k/v and
+gate/up as one matrix each; batches of many rows (prompts) dequantise a
+matrix and multiply.  `act_e4m3` hands the norms' rows on in 8 bits.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from collections.abc import Callable
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
 
 from . import _lib as L
-from . import paged
+from . import dense, paged
 
 
 @dataclass(frozen=True)
@@ -63,6 +70,11 @@ GEMMA_2B = DecoderShape(hidden=2048, layers=18, hq=8, hkv=1, head_dim=256, inter
                         gated_q=False, qk_norm=False, phantom=False, mlp="geglu")
 
 
+# Rows up to which the 4-bit matrix-vector product (which reads the weights once per 16 rows) beats dequantising
+# a matrix and multiplying.
+W4_MATVEC_ROWS = 64
+
+
 def _rms(x: torch.Tensor, w1: torch.Tensor, eps: float) -> torch.Tensor:
     """RmsNorm::forward (model.rs:98-108): x / sqrt(mean(x^2) + eps) * (1 + w), last axis; w1 = 1 + w."""
     return torch.nn.functional.rms_norm(x, (x.shape[-1],), w1, eps)
@@ -73,8 +85,14 @@ class QwenPagedModel:
 
     def __init__(self, shape: DecoderShape, weights: dict, num_pages: int, page_size: int = 16,
                  device: torch.device | str = "cuda", split_bf16: bool = True, dtype: torch.dtype = torch.float32,
-                 fused_prologue: bool = True, decode_plan: bool = True):
+                 fused_prologue: bool = True, decode_plan: bool = True, w4_group: int | None = None,
+                 act_e4m3: bool = False):
         self.s = shape
+        # w4_group: 4-bit weights with one scale per so many inputs (32, 64 or 128) for every matrix but the
+        # embedding lookup.  act_e4m3: the norms write e4m3 rows with a scale each for those matrices.
+        if act_e4m3 and w4_group is None:
+            raise ValueError("act_e4m3 needs 4-bit weights (w4_group)")
+        self.w4_group, self.act_e4m3 = w4_group, act_e4m3
         # Dense weights and activations in `dtype` (f32: the reference's CPU
         # path; bf16: the random-bf16 configs 3-5).  RoPE is applied in f32 and
         # the attention kernels take f32 q/k/v either way.
@@ -90,6 +108,11 @@ class QwenPagedModel:
         # (mtn_qkv_prologue) instead of torch ops and a separate append.
         self.fused = fused_prologue and shape.rotary_dim % 64 == 0
         self.w = {k: torch.as_tensor(v).to(self.dev, dtype) for k, v in weights.items()}
+        # (1 + w) of the layer norms in f32, and the 4-bit matrices
+        self.q4: dict[str, dense.W4Weight] = {}
+        self.w1: dict[str, torch.Tensor] = {}
+        if w4_group is not None:
+            self._quantize(w4_group)
         # RMSNorm scales (1 + w), formed once
         for k in [k for k in self.w if k.endswith("norm.weight")]:
             self.w[k] = self.w[k] + 1.0
@@ -112,7 +135,39 @@ class QwenPagedModel:
         self.use_plan = decode_plan
         self._graphs: dict[int, _DecodeGraph] = {}
 
+    def _quantize(self, group: int) -> None:
+        """Every matrix to 4 bits: q/k/v and gate/up stacked, the tied head from the embedding (which stays for lookups)."""
+        w = self.w
+        self.w1 = {k: (v.float() + 1.0).contiguous() for k, v in w.items() if k.endswith("norm.weight")}
+
+        def pack(name: str, *parts: str) -> None:
+            rows = [w.pop(f"{p}.weight") for p in parts]
+            self.q4[name] = dense.W4Weight.from_float(torch.cat(rows) if len(rows) > 1 else rows[0].contiguous(), group)
+
+        for li in range(self.s.layers):
+            p, m = f"layers.{li}", f"layers.{li}.mixer"
+            pack(f"{m}.qkv", f"{m}.q_proj", f"{m}.k_proj", f"{m}.v_proj")
+            pack(f"{m}.o_proj", f"{m}.o_proj")
+            pack(f"{p}.mlp.gate_up", f"{p}.mlp.gate_proj", f"{p}.mlp.up_proj")
+            pack(f"{p}.mlp.down_proj", f"{p}.mlp.down_proj")
+        self.q4["head"] = dense.W4Weight.from_float(w["embedding.weight"].contiguous(), group)
+
     # ------------------------------------------------------------ pieces
+    def _linear4(self, name: str, x: torch.Tensor, scales: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        """x @ W.T for a 4-bit matrix; x in the model's type, or e4m3 with a scale per row."""
+        w, out_dtype = self.q4[name], out_dtype or self.dt
+        if x.shape[0] <= W4_MATVEC_ROWS:
+            return dense.w4_matvec(x, w, x_scales=scales, out_dtype=out_dtype)
+        if scales is not None:
+            x = (x.float() * scales[:, None]).to(self.dt)
+        return (x @ w.dequantize(self.dt).T).to(out_dtype)
+
+    def _norm4(self, name: str, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """(rows, scales) of RMSNorm(x + residual), the sum left in `residual`."""
+        return dense.add_rms_norm(x, self.w1[f"{name}.weight"], self.s.eps, residual=residual,
+                                  out_dtype=torch.float8_e4m3fn if self.act_e4m3 else self.dt)
+
     def _rope_tables(self, pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """cos and sin of pos * inv_freq [T, 1, rotary_dim/2], shared by q, k and every layer."""
         ang = pos.to(torch.float32)[:, None, None] * self.inv_freq[None, None, :]
@@ -151,37 +206,44 @@ class QwenPagedModel:
             self._ws_seqs = n
         return self._ws
 
-    def _mlp(self, h: torch.Tensor, p: str) -> torch.Tensor:
-        g = h @ self.w[f"{p}.mlp.gate_proj.weight"].T
-        u = h @ self.w[f"{p}.mlp.up_proj.weight"].T
+    def _mlp(self, h: torch.Tensor, p: str, scales: torch.Tensor | None = None) -> torch.Tensor:
+        if self.w4_group is None:
+            g = h @ self.w[f"{p}.mlp.gate_proj.weight"].T
+            u = h @ self.w[f"{p}.mlp.up_proj.weight"].T
+        else:
+            g, u = self._linear4(f"{p}.mlp.gate_up", h, scales).split(self.s.inter, dim=1)
         act = torch.nn.functional.silu(g) if self.s.mlp == "swiglu" else torch.nn.functional.gelu(g, approximate="tanh")
+        if self.w4_group is not None:
+            return self._linear4(f"{p}.mlp.down_proj", act * u)
         return (act * u) @ self.w[f"{p}.mlp.down_proj.weight"].T
 
-    def _attention(self, li: int, h: torch.Tensor, cs: tuple[torch.Tensor, torch.Tensor], meta: dict) -> torch.Tensor:
+    def _attention(self, li: int, h: torch.Tensor, cs: tuple[torch.Tensor, torch.Tensor], meta: dict,
+                   scales: torch.Tensor | None = None) -> torch.Tensor:
         """GatedAttention::forward (model.rs:369-422) for every row of the batch."""
         s, w = self.s, self.w
         m = f"layers.{li}.mixer"
         T = h.shape[0]
-        qp = h @ w[f"{m}.q_proj.weight"].T
+        if self.w4_group is None:
+            qp, kp, vp = (h @ w[f"{m}.{x}_proj.weight"].T for x in "qkv")
+        else:
+            nq, nk = s.hq * s.head_dim * (2 if s.gated_q else 1), s.hkv * s.head_dim
+            qp, kp, vp = self._linear4(f"{m}.qkv", h, scales).split([nq, nk, nk], dim=1)
         if s.gated_q:
-            qg = qp.view(T, s.hq, 2, s.head_dim)  # per head: q then gate (model.rs:372-375)
+            qg = qp.unflatten(1, (s.hq, 2, s.head_dim))  # per head: q then gate (model.rs:372-375)
             q, gate = qg[:, :, 0, :], qg[:, :, 1, :].reshape(T, s.hq * s.head_dim)
         else:
-            q, gate = qp.view(T, s.hq, s.head_dim), None
-        k = (h @ w[f"{m}.k_proj.weight"].T).view(T, s.hkv, s.head_dim)
-        v = (h @ w[f"{m}.v_proj.weight"].T).view(T, s.hkv, s.head_dim)
+            q, gate = qp.unflatten(1, (s.hq, s.head_dim)), None
+        k, v = kp.unflatten(1, (s.hkv, s.head_dim)), vp.unflatten(1, (s.hkv, s.head_dim))
         attn = torch.empty((T, s.hq, s.head_dim), dtype=torch.float32, device=self.dev)
         tp = meta["tp"]
         if self.fused:
             # q/k norms, RoPE and every row's K/V store in one launch; the
             # attention kernels then find the step's rows in the pool
             q = torch.empty((T, s.hq, s.head_dim), dtype=torch.float32, device=self.dev)
-            qp = qp.contiguous()
-            kc, vc = k.contiguous(), v.contiguous()
             qw, kw = (self.w32.get(f"{m}.q_norm.weight"), self.w32.get(f"{m}.k_norm.weight")) if s.qk_norm else (None, None)
             L.check(L.lib().mtn_qkv_prologue(
-                paged.C.byref(self.pool.layout), li, qp.data_ptr(), kc.data_ptr(), vc.data_ptr(),
-                paged._dtype_code(self.dt), qp.shape[1], s.hkv * s.head_dim, s.hkv * s.head_dim, int(s.gated_q), s.hq,
+                paged.C.byref(self.pool.layout), li, qp.data_ptr(), kp.data_ptr(), vp.data_ptr(),
+                paged._dtype_code(self.dt), qp.stride(0), kp.stride(0), vp.stride(0), int(s.gated_q), s.hq,
                 None if qw is None else qw.data_ptr(), None if kw is None else kw.data_ptr(), s.eps,
                 self.inv_freq.data_ptr(), s.rotary_dim, meta["pos"].data_ptr(), meta["slots_all"].data_ptr(), T,
                 q.data_ptr(), paged._stream(None)))
@@ -206,6 +268,8 @@ class QwenPagedModel:
         o = attn.view(T, s.hq * s.head_dim).to(self.dt)
         if gate is not None:
             o = torch.sigmoid(gate) * o
+        if self.w4_group is not None:
+            return self._linear4(f"{m}.o_proj", o)
         return o @ w[f"{m}.o_proj.weight"].T
 
     # ------------------------------------------------------------ forward
@@ -255,12 +319,27 @@ class QwenPagedModel:
             cs = None
         else:
             cs = self._rope_tables(pos)
+        if self.w4_group is not None:
+            return self._layers4(x, cs, meta, last)
         for li in range(s.layers):
             p = f"layers.{li}"
             x = x + self._attention(li, _rms(x, w[f"{p}.norm.weight"], s.eps), cs, meta)
             x = x + self._mlp(_rms(x, w[f"{p}.ffn_norm.weight"], s.eps), p)
         h = _rms(x[last], w["norm.weight"], s.eps)
         return (h @ w["embedding.weight"].T).float().contiguous()  # tied LM head (model.rs:262-276)
+
+    def _layers4(self, x: torch.Tensor, cs, meta: dict, last: torch.Tensor) -> torch.Tensor:
+        """The layers and the head with 4-bit matrices: each residual sum and the norm behind it are one launch."""
+        s = self.s
+        h, sc = self._norm4("layers.0.norm", x)
+        for li in range(s.layers):
+            p = f"layers.{li}"
+            h, sc = self._norm4(f"{p}.ffn_norm", self._attention(li, h, cs, meta, sc), residual=x)
+            y = self._mlp(h, p, sc)
+            if li + 1 < s.layers:
+                h, sc = self._norm4(f"layers.{li + 1}.norm", y, residual=x)
+        h, sc = self._norm4("norm", y[last], residual=x[last])
+        return self._linear4("head", h, sc, out_dtype=torch.float32)
 
     @torch.no_grad()
     def forward(self, b) -> torch.Tensor:
@@ -351,6 +430,17 @@ class _DecodeGraph:
         return res
 
 
+@dataclass
+class TokenRules:
+    """What a request asks of its logits before a token is picked (paged.LogitsRules for one row)."""
+    repetition: float = 1.0   # > 0: divides positive, multiplies negative logits of every token so far
+    presence: float = 0.0     # subtracted once from every generated token
+    frequency: float = 0.0    # subtracted per occurrence among the generated tokens
+    bias: dict[int, float] = field(default_factory=dict)
+    # generated tokens so far -> [vocab] truth values of the tokens allowed next, or None for all
+    allowed: Callable[[list[int]], np.ndarray | None] | None = None
+
+
 class Engine:
     """engine_loop.rs:28-107 over the scheduler mirror and a paged model.
 
@@ -359,7 +449,8 @@ class Engine:
     temperature (sample_token, scheduler.rs:186-223: greedy first strict max
     or the reference's hash-of-logits pick) and hand the tokens back to the
     scheduler.  A backend error aborts every request of the batch
-    (engine_loop.rs:47-57).
+    (engine_loop.rs:47-57).  Requests with token rules (set_rules) have their
+    rows processed first (mtn_process_logits).
     """
 
     def __init__(self, model: QwenPagedModel, sched, cuda_graphs: bool = True):
@@ -367,6 +458,70 @@ class Engine:
         self.cuda_graphs = cuda_graphs
         self.iterations = 0
         self._sample_ws = None
+        self._rules: dict[int, tuple[np.ndarray, TokenRules]] = {}
+        self._rules_ws = None
+
+    def set_rules(self, req_id: int, prompt, rules: TokenRules) -> None:
+        """Penalties, biases and masks for a queued request; `prompt` is what it was queued with."""
+        vocab = self.model.s.vocab
+        ids = np.asarray(prompt, dtype=np.int64)
+        if ids.ndim != 1 or ids.size and (ids.min() < 0 or ids.max() >= vocab):
+            raise ValueError("prompt must be a list of token ids of the vocabulary")
+        if not rules.repetition > 0 or not np.isfinite([rules.repetition, rules.presence, rules.frequency]).all():
+            raise ValueError("repetition must be positive, and the penalties finite")
+        if any(not 0 <= t < vocab for t in rules.bias) or np.isnan(list(rules.bias.values())).any():
+            raise ValueError("bias: token ids of the vocabulary with values that are numbers")
+        self._rules[int(req_id)] = (ids.astype(np.int32), rules)
+
+    def _apply_rules(self, b, logits: torch.Tensor, greedy: bool) -> torch.Tensor | None:
+        """The batch's rules on its logits, in place; the greedy tokens if asked for.  Rows without rules pass as
+        they are."""
+        n, vocab = logits.shape
+        mine = [self._rules.get(int(r)) for r in b.req_ids]
+        out = [self.sched.request_output(int(r)) if m else [] for r, m in zip(b.req_ids, mine)]
+        none = (np.zeros(0, np.int32), TokenRules())
+        hist = [np.concatenate([m[0], np.asarray(o, np.int32)]) if m else none[0] for m, o in zip(mine, out)]
+        rules = [(m or none)[1] for m in mine]
+        dev = logits.device
+
+        def up(a, dtype):
+            return torch.from_numpy(np.ascontiguousarray(a, dtype)).to(dev)
+
+        def indptr(lens):
+            return up(np.concatenate([[0], np.cumsum(lens)]), np.int32)
+
+        kw = {"hist_indptr": indptr([len(h) for h in hist]), "hist_tokens": up(np.concatenate(hist), np.int32),
+              "prompt_lens": up([len(m[0]) if m else 0 for m in mine], np.int32),
+              "repetition": up([r.repetition for r in rules], np.float32),
+              "presence": up([r.presence for r in rules], np.float32),
+              "frequency": up([r.frequency for r in rules], np.float32)}
+        if any(r.bias for r in rules):
+            kw["bias_indptr"] = indptr([len(r.bias) for r in rules])
+            kw["bias_tokens"] = up([t for r in rules for t in r.bias], np.int32)
+            kw["bias_values"] = up([v for r in rules for v in r.bias.values()], np.float32)
+        masks, rows = [], []
+        for r, o in zip(rules, out):
+            allow = r.allowed(o) if r.allowed is not None else None
+            rows.append(-1 if allow is None else len(masks))
+            if allow is not None:
+                allow = np.asarray(allow, dtype=bool)
+                if allow.shape != (vocab,):
+                    raise ValueError(f"allowed() must give {vocab} truth values")
+                bits = np.zeros(-(-vocab // 32) * 32, np.uint8)
+                bits[:vocab] = allow
+                masks.append(np.packbits(bits, bitorder="little").view(np.int32))
+        if masks:
+            kw["mask"], kw["mask_rows"] = up(np.stack(masks), np.int32), up(rows, np.int32)
+        if greedy and (self._rules_ws is None or self._rules_ws.numel() < 16 * n):
+            self._rules_ws = paged.logits_workspace(n, dev)
+        return paged.process_logits(logits, paged.LogitsRules(**kw), out=logits, greedy=greedy,
+                                    workspace=self._rules_ws)[1]
+
+    def _drop_rules(self, b) -> None:
+        """Forget the rules of requests that have ended."""
+        for r in b.req_ids:
+            if int(r) in self._rules and self.sched.request_info(int(r))["state"] in (L.MTN_REQ_DONE, L.MTN_REQ_ABORTED):
+                del self._rules[int(r)]
 
     def step(self) -> bool:
         b = self.sched.schedule()
@@ -374,14 +529,21 @@ class Engine:
             return False
         try:
             logits = self.model.decode_step(b) if self.cuda_graphs else self.model.forward(b)
-            if np.any(b.temperatures > 0):
+            hot = bool(np.any(b.temperatures > 0))
+            picked = None
+            if any(int(r) in self._rules for r in b.req_ids):
+                try:
+                    picked = self._apply_rules(b, logits, not hot)
+                except Exception as e:  # a request's allowed() is the caller's code
+                    raise RuntimeError("the batch's token rules could not be applied") from e
+            if hot:
                 nb = L.lib().mtn_sample_rows_workspace_bytes(*logits.shape)
                 if self._sample_ws is None or self._sample_ws.numel() < nb:
                     self._sample_ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
                 temps = torch.from_numpy(b.temperatures).to(logits.device)
                 tokens = paged.sample_rows(logits, temps, workspace=self._sample_ws).cpu().numpy().astype(np.uint32)
             else:
-                tokens = paged.argmax_rows(logits).cpu().numpy().astype(np.uint32)
+                tokens = (paged.argmax_rows(logits) if picked is None else picked).cpu().numpy().astype(np.uint32)
             code, detail = paged.device_error(self.model.dev.index or 0)
             if code:
                 timeout = code == paged.DEV_ERR_TIMEOUT
@@ -391,8 +553,11 @@ class Engine:
                                     f"device error {code} (detail {detail}) in the step's kernels")
         except (L.MittenError, RuntimeError):
             self.sched.abort_batch()
+            self._drop_rules(b)
             raise
         self.sched.process_tokens(tokens)
+        if self._rules:
+            self._drop_rules(b)
         self.iterations += 1
         return True
 
