@@ -121,31 +121,58 @@ __global__ void __launch_bounds__(128) w4_pack_kernel(const void* w, int dtype, 
   }
 }
 
-// Row-major values q * s of 16 rows x 128 k per CTA; the product of a 4-bit
-// integer and a bf16 scale is exact in f32 and rounded once for bf16.
-__global__ void __launch_bounds__(128) w4_dequantize_kernel(const uint4* packed, const uint32_t* scales, int64_t n,
-                                                            int64_t k, int group, void* out, int dtype,
-                                                            int64_t stride) {
-  const int64_t ksteps = pad_k(k) / kKPad;
-  const int64_t ru = blockIdx.x / ksteps, ks = blockIdx.x - ru * ksteps;
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(packed + (ru * ksteps + ks) * 64);
-  const int j = threadIdx.x;
-  const int64_t col = ks * kKPad + j;
-  if (col >= k) return;
-  const int gpw = kKPad / group;
-  const int u = j >> 6, h = (j >> 5) & 1, t = (j >> 3) & 3;
-  for (int r = 0; r < kRowUnit; ++r) {
-    const int64_t row = ru * kRowUnit + r;
-    if (row >= n) return;
-    const int g = r & 7;
-    const uint32_t w = words[(u * 32 + 4 * g + t) * 4 + (r >> 3) * 2 + h];
-    const uint32_t s2 = scales[((ru * ksteps + ks) * gpw + j / group) * 8 + g];
-    const float s = __uint_as_float(r >= 8 ? s2 & 0xffff0000u : s2 << 16);
-    const float v = static_cast<float>(code_of(w, j & 7)) * s;
-    if (dtype == MTN_DTYPE_BF16)
-      static_cast<__nv_bfloat16*>(out)[row * stride + col] = __float2bfloat16_rn(v);
-    else
-      static_cast<float*>(out)[row * stride + col] = v;
+// Row-major values q * s, 16 rows x 128 k at a time, kDequantSteps of them per
+// CTA; a thread has eight consecutive k of a row.  The product of a 4-bit
+// integer and a bf16 scale is exact in f32 and rounded once for bf16.  Bound by
+// the bytes written.
+constexpr int kDequantSteps = 4;
+
+__global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* packed, const uint32_t* scales, int64_t n,
+                                                            int64_t k, int group, void* out, int dtype, int64_t stride,
+                                                            bool vec) {
+  const int64_t ksteps = pad_k(k) / kKPad, blocks = (ksteps + kDequantSteps - 1) / kDequantSteps;
+  const int64_t ru = blockIdx.x / blocks, first = (blockIdx.x - ru * blocks) * kDequantSteps;
+  const int r = threadIdx.x >> 4, c = threadIdx.x & 15, g = r & 7;
+  const int64_t row = ru * kRowUnit + r;
+  if (row >= n) return;
+  const int word = (((c >> 3) * 32 + 4 * g + (c & 3)) * 4) + (r >> 3) * 2 + ((c >> 2) & 1), gpw = kKPad / group;
+  uint32_t w[kDequantSteps], s2[kDequantSteps];
+#pragma unroll
+  for (int i = 0; i < kDequantSteps; ++i) {
+    const int64_t at = ru * ksteps + first + i;
+    if (first + i < ksteps) {
+      w[i] = packed[at * 256 + word];
+      s2[i] = scales[(at * gpw + c * 8 / group) * 8 + g];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kDequantSteps; ++i) {
+    const int64_t col = (first + i) * kKPad + c * 8;
+    if (col >= k) return;
+    const float s = __uint_as_float(r >= 8 ? s2[i] & 0xffff0000u : s2[i] << 16);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(code_of(w[i], j)) * s;
+    const int64_t to = row * stride + col;
+    if (vec && col + 8 <= k) {
+      if (dtype == MTN_DTYPE_BF16) {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to) =
+            make_uint4(f2_to_bf2(v[0], v[1]), f2_to_bf2(v[2], v[3]), f2_to_bf2(v[4], v[5]), f2_to_bf2(v[6], v[7]));
+      } else {
+        float4* q = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
+        q[0] = make_float4(v[0], v[1], v[2], v[3]);
+        q[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (col + j >= k) break;
+      if (dtype == MTN_DTYPE_BF16)
+        static_cast<__nv_bfloat16*>(out)[to + j] = __float2bfloat16_rn(v[j]);
+      else
+        static_cast<float*>(out)[to + j] = v[j];
+    }
   }
 }
 
@@ -663,18 +690,20 @@ __global__ void __launch_bounds__(kMvThreads, 1) w4_matvec_kernel(const W4Params
       }
       cluster_sync();
     } else {
-      // Join a unit that begins in this warp and goes on in the next ones.
+      // Join the units that begin in a warp and go on in the next ones.
+      __shared__ int tail_of[kMvWarps];
+      const int i1 = i0 + n_items, tail = i1 / L;
+      if (lane == 0) tail_of[warp] = n_items > 0 && i1 != tail * L && tail * L >= i0 ? tail : -1;
       __syncthreads();
-      const int i1 = i0 + n_items, q = i1 / L;
-      if (n_items > 0 && i1 != q * L && q * L >= i0) {
-        const float* tail = reinterpret_cast<const float*>(ring_ptr);
-        for (int i = lane; i < mt * kUnitRows; i += 32) {
-          float v = tail[i];
-          for (int z = warp + 1; z < kMvWarps && z * total / kMvWarps < (q + 1) * L; ++z)
-            if (z * total / kMvWarps != (z + 1) * total / kMvWarps) v += slots[z * kSlot + i];
-          const int64_t n = static_cast<int64_t>(u0 + q) * kUnitRows + i % kUnitRows;
-          if (n < p.n) store_out(p, m0 + i / kUnitRows, n, v);
-        }
+      const int per_unit = mt * kUnitRows;
+      for (int e = tid; e < (kMvWarps - 1) * per_unit; e += kMvThreads) {
+        const int w = e / per_unit, i = e - w * per_unit, q = tail_of[w], m = i / kUnitRows;
+        if (q < 0) continue;
+        float v = reinterpret_cast<const float*>(smem + plan.ring_off + w * (kD * kStage))[i];
+        for (int z = w + 1; z < kMvWarps && z * total / kMvWarps < (q + 1) * L; ++z)
+          if (z * total / kMvWarps != (z + 1) * total / kMvWarps) v += slots[z * kSlot + i];
+        const int64_t n = static_cast<int64_t>(u0 + q) * kUnitRows + i % kUnitRows;
+        if (n < p.n) store_out(p, m0 + m, n, v);
       }
       if (u0 + nu < cu1) __syncthreads();
     }
@@ -850,9 +879,12 @@ int mtn_w4_dequantize(const void* packed, const void* scales, int64_t n, int64_t
   MTN_CHECK_ARG(dtype == MTN_DTYPE_BF16 || dtype == MTN_DTYPE_F32, "mtn_w4_dequantize: bad dtype");
   MTN_CHECK_ARG(stride >= k, "mtn_w4_dequantize: row stride shorter than a row");
   MTN_CHECK_ARG(mtn::aligned16(packed) && mtn::aligned16(scales), "mtn_w4_dequantize: packed and scales must be 16-byte aligned");
-  const int64_t blocks = mtn::row_units(n) * (mtn::pad_k(k) / mtn::kKPad);
-  mtn::w4_dequantize_kernel<<<static_cast<unsigned>(blocks), 128, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint4*>(packed), static_cast<const uint32_t*>(scales), n, k, group, out, dtype, stride);
+  const int64_t ksteps = mtn::pad_k(k) / mtn::kKPad;
+  const int64_t blocks = mtn::row_units(n) * ((ksteps + mtn::kDequantSteps - 1) / mtn::kDequantSteps);
+  const int elem = dtype == MTN_DTYPE_BF16 ? 2 : 4;
+  const bool vec = mtn::aligned16(out) && (n == 1 || stride * elem % 16 == 0);
+  mtn::w4_dequantize_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(packed), static_cast<const uint32_t*>(scales), n, k, group, out, dtype, stride, vec);
   return mtn::check_launch("w4_dequantize_kernel");
 }
 
