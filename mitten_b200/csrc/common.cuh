@@ -28,6 +28,12 @@ int cuda_status(cudaError_t e, const char* what);
     if (_e != cudaSuccess) return ::mtn::cuda_status(_e, what); \
   } while (0)
 
+// Whether a pointer (or null) is aligned to elements of an MTN_DTYPE_*.
+inline bool elem_aligned(const void* p, int dtype) {
+  const uintptr_t size = dtype == MTN_DTYPE_F32 ? 4 : dtype == MTN_DTYPE_BF16 ? 2 : 1;
+  return reinterpret_cast<uintptr_t>(p) % size == 0;
+}
+
 // Launch-result check after a <<<>>> launch.
 int check_launch(const char* what);
 

@@ -449,6 +449,8 @@ int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, in
   MTN_CHECK_ARG(row_stride >= vocab && out_stride >= vocab, "mtn_process_logits: row strides shorter than a row");
   MTN_CHECK_ARG(static_cast<const void*>(out) != logits || (dtype == MTN_DTYPE_F32 && row_stride == out_stride),
                 "mtn_process_logits: in place needs f32 logits and equal strides");
+  MTN_CHECK_ARG(mtn::elem_aligned(logits, dtype) && mtn::elem_aligned(out, MTN_DTYPE_F32),
+                "mtn_process_logits: a pointer is not aligned to its elements");
   const mtn_logits_rules& r = *rules;
   MTN_CHECK_ARG(r.n_hist >= 0 && r.n_hist <= INT32_MAX && r.n_bias >= 0 && r.n_bias <= INT32_MAX,
                 "mtn_process_logits: bad list sizes");

@@ -903,6 +903,9 @@ int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float*
                 "mtn_w4_matvec: x_scales go with e4m3 rows, and only with them");
   MTN_CHECK_ARG(x_stride >= k && out_stride >= n, "mtn_w4_matvec: row strides shorter than a row");
   MTN_CHECK_ARG(mtn::aligned16(packed) && mtn::aligned16(scales), "mtn_w4_matvec: packed and scales must be 16-byte aligned");
+  MTN_CHECK_ARG(mtn::elem_aligned(x, x_dtype) && mtn::elem_aligned(out, out_dtype) &&
+                    mtn::elem_aligned(x_scales, MTN_DTYPE_F32),
+                "mtn_w4_matvec: a pointer is not aligned to its elements");
   MTN_CHECK_ARG(out != x, "mtn_w4_matvec: out overlaps x");
   mtn::W4Params p{x, x_dtype, x_stride, x_scales, n_rows, static_cast<const uint4*>(packed),
                   static_cast<const uint32_t*>(scales), n, k, group, out, out_dtype, out_stride};

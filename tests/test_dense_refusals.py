@@ -38,6 +38,9 @@ def _norm(x=FAKE[0], x_dtype=_lib.MTN_DTYPE_BF16, x_stride=64, residual=FAKE[1],
     (dict(x_stride=63), b"strides"),
     (dict(out_stride=63), b"strides"),
     (dict(sum_stride=63), b"strides"),
+    (dict(x=C.c_void_p(0x100001)), b"not aligned"),
+    (dict(out=C.c_void_p(0x400002), out_dtype=_lib.MTN_DTYPE_F32), b"not aligned"),
+    (dict(w1=C.c_void_p(0x500002)), b"not aligned"),
 ])
 def test_norm_refuses(kw, msg):
     assert _norm(**kw) == _lib.MTN_EINVAL
@@ -68,6 +71,7 @@ def _matvec(x=FAKE[0], x_dtype=_lib.MTN_DTYPE_BF16, x_stride=128, xs=None, m=2, 
     (dict(x_stride=127), b"strides"), (dict(out_stride=31), b"strides"),
     (dict(packed=C.c_void_p(0x100008)), b"aligned"), (dict(scales=C.c_void_p(0x100004)), b"aligned"),
     (dict(out=FAKE[0]), b"overlaps"),
+    (dict(x=C.c_void_p(0x100001)), b"not aligned"), (dict(out=C.c_void_p(0x400002)), b"not aligned"),
 ])
 def test_w4_matvec_refuses(kw, msg):
     assert _matvec(**kw) == _lib.MTN_EINVAL

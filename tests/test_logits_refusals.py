@@ -20,6 +20,7 @@ def _call(rules=None, no_rules=False, logits=P[0], dtype=_lib.MTN_DTYPE_F32, str
 @pytest.mark.parametrize("kw,msg", [
     (dict(n=-1), b"bad sizes"), (dict(vocab=0), b"bad sizes"), (dict(dtype=_lib.MTN_DTYPE_E4M3), b"bad dtype"),
     (dict(logits=None), b"null"), (dict(out=None), b"null"), (dict(no_rules=True), b"null"),
+    (dict(logits=P[0] + 2), b"not aligned"), (dict(out=P[1] + 2), b"not aligned"),
     (dict(stride=99), b"strides"), (dict(out_stride=99), b"strides"),
     (dict(out=P[0], dtype=_lib.MTN_DTYPE_BF16), b"in place"), (dict(out=P[0], out_stride=128), b"in place"),
     (dict(rules=dict(n_hist=-1)), b"list sizes"), (dict(rules=dict(hist_indptr=P[2], n_hist=3)), b"hist_tokens"),
