@@ -19,9 +19,10 @@
 // load; that pass is bound by memory and needs nothing of the first kernel,
 // which therefore runs beside it (programmatic dependent launch).  Then it
 // waits, counts its entries in a table in shared memory (integer atomics, so
-// nothing depends on their order) and applies penalties and biases to the
-// original logits, the first entry to claim a token doing its work; a thread
-// whose maximum is a touched element looks its elements over again.  The
+// nothing depends on their order), and the first entry to claim a token
+// applies its penalties to the original logit; the biases go the same way over
+// the same table.  A thread whose maximum is a touched element looks its
+// elements over again.  The
 // chunks of a row join their maxima as 64-bit keys (value, then lowest index)
 // with an atomic maximum; the last one to arrive writes the token and leaves
 // the workspace zeroed.
@@ -31,7 +32,9 @@
 // over a cluster's distributed shared memory (56-70 us: a frequent token's
 // remote atomics queue up), one CTA per row making a list of different tokens
 // in a hash table (45 us; 170 us for 128 x 256000, where a row's 13 k different
-// tokens keep one SM busy for 100 us).
+// tokens keep one SM busy for 100 us), the rules in a third kernel of a small
+// CTA per 4096 tokens (51 us: its chains of small loads take longer than the
+// pass over the logits that they hide behind here).
 #include <algorithm>
 
 #include "common.cuh"
@@ -40,11 +43,15 @@ namespace mtn {
 namespace {
 
 constexpr int kLogitsThreads = 256;
-constexpr int kLogitsResident = 8;  // CTAs an SM holds, by registers (with 4 and twice the loads: 40.2 us, with 6: 38)
+// CTAs an SM holds, by registers.  With rules, 64 x 152064 took 32.2, 32.7 and
+// 36.4 us with 8, 6 and 4 (and more loads ahead); with a mask alone 21.9, 18.0
+// and 19.5.
+constexpr int logits_resident(bool rules) { return rules ? 8 : 6; }
 constexpr int kChunkStep = 1024, kChunkMax = 32768;
 constexpr int kChunkMaxRuled = 8192;  // tables of 32 KB
 constexpr int kChunkFixed = 2048;
 constexpr int kBatchVecs = 2;         // 16-byte loads of a thread ahead of the ones in work
+constexpr int kAhead = 4;             // list entries of a thread in flight
 constexpr int kSortThreads = 1024;
 constexpr int kBuckets = 512;         // a row's chunks, or groups of 2^k of them
 constexpr uint32_t kGenerated = 0x80000000u;
@@ -99,7 +106,6 @@ __device__ __forceinline__ int row_head(const LogitsParams& p, int row) {
 template <typename F>
 __device__ __forceinline__ void sort_list(const LogitsParams& p, int row, int head, const int32_t* tokens, int64_t beg,
                                           int64_t end, int32_t* starts, int* count, F place) {
-  constexpr int kAhead = 4;
   const int tid = threadIdx.x, lane = tid & 31;
   const uint32_t vocab = static_cast<uint32_t>(p.vocab);
   auto bucket_of = [&](int32_t t) {
@@ -204,13 +210,15 @@ __device__ __forceinline__ float ld_logit(const T* p) {
 
 // kHist, kBias: a history, biases are given, and sort_rules_kernel went before.
 template <typename T, bool kHist, bool kBias>
-__global__ void __launch_bounds__(kLogitsThreads, kLogitsResident) process_logits_kernel(const LogitsParams p) {
+__global__ void __launch_bounds__(kLogitsThreads, logits_resident(kHist || kBias)) process_logits_kernel(const LogitsParams p) {
   extern __shared__ __align__(16) uint32_t smem[];
   constexpr int kN = Vec<T>::kN;
   constexpr bool kRules = kHist || kBias;
   const int tid = threadIdx.x;
-  const int row = static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.chunks));
-  const int chunk = static_cast<int>(blockIdx.x - static_cast<uint32_t>(row) * p.chunks), vocab = static_cast<int>(p.vocab);
+  // The first chunks of all rows first: a tokenizer's frequent tokens come
+  // early, and so do the chunks with the most entries.
+  const int chunk = static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.n_rows));
+  const int row = static_cast<int>(blockIdx.x - static_cast<uint32_t>(chunk) * p.n_rows), vocab = static_cast<int>(p.vocab);
   const T* in = static_cast<const T*>(p.logits) + row * p.row_stride;
   float* out = p.out + row * p.out_stride;
   // Chunks begin where a 16-byte load may: `head` elements into the row; the
@@ -303,12 +311,14 @@ __global__ void __launch_bounds__(kLogitsThreads, kLogitsResident) process_logit
 
   unsigned long long key = 0;
   if constexpr (kRules) {
-    // shared memory: a bitmap of touched elements; times generated, and
-    // kGenerated for being in the history at all; index + 1 of the last bias
+    // shared memory: bitmaps of touched elements and of those with a bias; a
+    // table of times generated, and kGenerated for being in the history at
+    // all, then of index + 1 of a token's last bias
+    const int map_words = p.size / 32 + 4;
     uint32_t* touched = smem;
-    uint32_t* count = smem + p.size / 32 + 4;
-    uint32_t* bias = count + (kHist ? p.size + 8 : 0);
-    const int vecs = static_cast<int>(bias - smem + (kBias ? p.size + 8 : 0)) / 4;
+    uint32_t* biased = touched + map_words;
+    uint32_t* table = biased + (kBias ? map_words : 0);
+    const int vecs = static_cast<int>(table - smem + p.size + 8) / 4;
     for (int i = tid; i < vecs; i += kLogitsThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     int64_t hbeg = 0, bbeg = 0, end;
     if constexpr (kHist) row_range(p.r.hist_indptr, row, p.r.n_hist, hbeg, end, p.err);
@@ -331,45 +341,84 @@ __global__ void __launch_bounds__(kLogitsThreads, kLogitsResident) process_logit
       n_bias = p.sorted.bias_starts[bucket + 1] - from;
       bias_list = p.sorted.bias + bbeg + from;
     }
+    // Calls f for kAhead history entries at a time: places of the chunk, and
+    // kNone where there is no entry or it is another chunk's of the bucket;
+    // kGenerated with a place as with its entry.
+    constexpr uint32_t kNone = ~kGenerated;
+    auto entries = [&](auto f) {
+      for (int i = tid; i < n_hist; i += kAhead * kLogitsThreads) {
+        uint32_t k[kAhead];
+#pragma unroll
+        for (int b = 0; b < kAhead; ++b) k[b] = i + b * kLogitsThreads < n_hist ? hist_list[i + b * kLogitsThreads] : kNone;
+#pragma unroll
+        for (int b = 0; b < kAhead; ++b) {
+          const uint32_t at = (k[b] & ~kGenerated) - static_cast<uint32_t>(v0);
+          k[b] = k[b] != kNone && at < static_cast<uint32_t>(nv) ? at | (k[b] & kGenerated) : kNone;
+        }
+        f(k);
+      }
+    };
     __syncthreads();  // the tables, and the first pass's stores
-    for (int i = tid; i < n_hist; i += kLogitsThreads) {
-      const uint32_t t = hist_list[i], k = (t & ~kGenerated) - static_cast<uint32_t>(v0);
-      if (k >= static_cast<uint32_t>(nv)) continue;  // another chunk of the bucket
-      if (!(count[k] & kGenerated)) atomicOr(&count[k], kGenerated);
-      if (t & kGenerated) atomicAdd(&count[k], 1u);
-    }
+    entries([&](const uint32_t(&k)[kAhead]) {
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        if (k[b] == kNone) continue;
+        uint32_t* slot = &table[k[b] & ~kGenerated];
+        if (!(*slot & kGenerated)) atomicOr(slot, kGenerated);
+        if (k[b] & kGenerated) atomicAdd(slot, 1u);
+      }
+    });
     for (int i = tid; i < n_bias; i += kLogitsThreads) {
       const uint32_t k = bias_list[i].x - static_cast<uint32_t>(v0);
-      if (k < static_cast<uint32_t>(nv)) atomicMax(&bias[k], bias_list[i].y + 1u);
+      if (k < static_cast<uint32_t>(nv)) atomicOr(&biased[k >> 5], 1u << (k & 31));
     }
     __syncthreads();
-    // The first entry to take a token's counts out of the tables applies them.
-    auto apply = [&](uint32_t k, uint32_t in_hist, uint32_t in_bias) {
-      atomicOr(&touched[k >> 5], 1u << (k & 31));
-      if (!allowed(k)) return;
-      float y = ld_logit(in + k);
-      if (in_hist != 0) {
-        const uint32_t n = in_hist & ~kGenerated;
-        y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-        y = __fsub_rn(y, __fmul_rn(freq, static_cast<float>(n)));
-        if (n != 0) y = __fsub_rn(y, pres);
+    // The first entry to take a token's count out of the table applies it.
+    entries([&](const uint32_t(&e)[kAhead]) {
+      uint32_t c[kAhead];
+      float y[kAhead];
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        const uint32_t k = e[b] & ~kGenerated;
+        c[b] = e[b] != kNone && table[k] != 0 ? atomicExch(&table[k], 0u) : 0u;
+        if (c[b] == 0) continue;
+        atomicOr(&touched[k >> 5], 1u << (k & 31));
+        if (!allowed(static_cast<int>(k))) c[b] = 0;
       }
-      if (in_bias != 0) y = __fadd_rn(y, p.r.bias_values[bbeg + in_bias - 1]);
-      out[k] = y;
-      key = max(key, arg_key(y, v0 + static_cast<int>(k)));
-    };
-    for (int i = tid; i < n_hist; i += kLogitsThreads) {
-      const uint32_t k = (hist_list[i] & ~kGenerated) - static_cast<uint32_t>(v0);
-      if (k >= static_cast<uint32_t>(nv) || count[k] == 0) continue;
-      const uint32_t c = atomicExch(&count[k], 0u);
-      if (c != 0) apply(k, c, kBias ? atomicExch(&bias[k], 0u) : 0u);
-    }
-    if (kHist && kBias) __syncthreads();
-    for (int i = tid; i < n_bias; i += kLogitsThreads) {
-      const uint32_t k = bias_list[i].x - static_cast<uint32_t>(v0);
-      if (k >= static_cast<uint32_t>(nv)) continue;
-      const uint32_t b = atomicExch(&bias[k], 0u);
-      if (b != 0) apply(k, 0u, b);
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b)
+        if (c[b] != 0) y[b] = ld_logit(in + (e[b] & ~kGenerated));
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        if (c[b] == 0) continue;
+        const uint32_t k = e[b] & ~kGenerated, n = c[b] & ~kGenerated;
+        float z = y[b] > 0.0f ? __fdiv_rn(y[b], rep) : __fmul_rn(y[b], rep);
+        z = __fsub_rn(z, __fmul_rn(freq, static_cast<float>(n)));
+        if (n != 0) z = __fsub_rn(z, pres);
+        out[k] = z;
+        if (!kBias || !(biased[k >> 5] >> (k & 31) & 1u)) key = max(key, arg_key(z, v0 + static_cast<int>(k)));
+      }
+    });
+    if constexpr (kBias) {
+      __syncthreads();  // the table is zero again, the penalties are stored
+      if (n_bias > 0) {
+        for (int i = tid; i < n_bias; i += kLogitsThreads) {
+          const uint32_t k = bias_list[i].x - static_cast<uint32_t>(v0);
+          if (k < static_cast<uint32_t>(nv)) atomicMax(&table[k], bias_list[i].y + 1u);
+        }
+        __syncthreads();
+        for (int i = tid; i < n_bias; i += kLogitsThreads) {
+          const uint32_t k = bias_list[i].x - static_cast<uint32_t>(v0);
+          if (k >= static_cast<uint32_t>(nv)) continue;
+          const uint32_t last = atomicExch(&table[k], 0u);
+          if (last == 0) continue;
+          const bool penalised = (atomicOr(&touched[k >> 5], 1u << (k & 31)) >> (k & 31) & 1u) != 0;
+          if (!allowed(static_cast<int>(k))) continue;
+          const float y = __fadd_rn(penalised ? out[k] : ld_logit(in + k), p.r.bias_values[bbeg + last - 1]);
+          out[k] = y;
+          key = max(key, arg_key(y, v0 + static_cast<int>(k)));
+        }
+      }
     }
     __syncthreads();
     auto is_touched = [&](int k) { return (touched[k >> 5] >> (k & 31) & 1u) != 0; };
@@ -420,7 +469,7 @@ LogitsKernel logits_kernel(bool hist, bool biased) {
 
 // Shared memory of a chunk of `size` elements, bytes.
 constexpr int logits_smem(int size, bool hist, bool biased) {
-  return hist || biased ? (size / 32 + 4 + (static_cast<int>(hist) + static_cast<int>(biased)) * (size + 8)) * 4 : 0;
+  return hist || biased ? ((size / 32 + 4) * (biased ? 2 : 1) + size + 8) * 4 : 0;
 }
 
 }  // namespace
@@ -482,8 +531,9 @@ int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, in
   const bool hist = n_hist > 0, biased = n_bias > 0;
   for (int sz = mtn::kChunkStep; sz <= (ruled ? mtn::kChunkMaxRuled : mtn::kChunkMax); sz += mtn::kChunkStep) {
     const int64_t c = (vocab + sz - 1) / sz;
-    const int fit = ruled ? 227 * 1024 / (mtn::logits_smem(sz, hist, biased) + 1024) : mtn::kLogitsResident;
-    const int64_t slots = static_cast<int64_t>(mtn::sm_count()) * std::min(fit, mtn::kLogitsResident);
+    const int most = mtn::logits_resident(ruled);
+    const int fit = ruled ? std::min(most, 227 * 1024 / (mtn::logits_smem(sz, hist, biased) + 1024)) : most;
+    const int64_t slots = static_cast<int64_t>(mtn::sm_count()) * fit;
     const int64_t cost = (n_rows * c + slots - 1) / slots * (sz + mtn::kChunkFixed);
     if (cost < best) {
       best = cost;
