@@ -27,6 +27,11 @@
 // with an atomic maximum; the last one to arrive writes the token and leaves
 // the workspace zeroed.
 //
+// 64 x 152064 f32 with histories of 2048 tokens on average, 32 biases and a
+// mask takes 32 us, the mask alone 18 (4.4 TB/s, 0.67 of the copy rate); the
+// difference is the chain of small loads behind the pass, of which a wave of
+// CTAs has one.  128 x 256000 bf16 with 8192 tokens: 81 us, the mask alone 41.
+//
 // Not kept, for 64 x 152064 with everything on: every chunk counting over the
 // whole history (50 us: most warp steps met a hit for a lane or two), counting
 // over a cluster's distributed shared memory (56-70 us: a frequent token's
