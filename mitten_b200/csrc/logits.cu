@@ -419,7 +419,9 @@ __global__ void __launch_bounds__(kLogitsThreads, logits_resident(kHist || kBias
           if (last == 0) continue;
           const bool penalised = (atomicOr(&touched[k >> 5], 1u << (k & 31)) >> (k & 31) & 1u) != 0;
           if (!allowed(static_cast<int>(k))) continue;
-          const float y = __fadd_rn(penalised ? out[k] : ld_logit(in + k), p.r.bias_values[bbeg + last - 1]);
+          // a malformed index pointer may have rows that share entries, and another row's index here
+          const float bias = p.r.bias_values[min(bbeg + last, p.r.n_bias) - 1];
+          const float y = __fadd_rn(penalised ? out[k] : ld_logit(in + k), bias);
           out[k] = y;
           key = max(key, arg_key(y, v0 + static_cast<int>(k)));
         }

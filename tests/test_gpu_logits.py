@@ -218,6 +218,23 @@ def test_bad_entries_are_skipped_and_reported(cuda_device):
     assert paged.device_error(0) == (0, 0)
 
 
+def test_rows_that_share_entries_read_only_their_list(cuda_device):
+    # rows 0 and 2 of an index pointer that falls share entries 50..99: their values are undefined, but what they
+    # add is a bias of the list, and row 3 is as it should be
+    n = 100
+    indptr = torch.tensor([0, n, n // 2, n, n + 1], dtype=torch.int32, device="cuda")
+    tokens = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    store = torch.full((4 * n,), float("nan"), device="cuda")
+    store[:n + 1] = 1.0
+    x = torch.zeros(4, 1000, device="cuda")
+    rules = paged.LogitsRules(bias_indptr=indptr, bias_tokens=tokens, bias_values=store[:n + 1])
+    for _ in range(20):
+        out, _ = paged.process_logits(x, rules)
+        assert paged.device_error(0)[0] == 7
+        assert ((out == 0) | (out == 1)).all() and not out[1].any()
+        assert out[3].nonzero().tolist() == [[n]]
+
+
 def test_streams_replay_and_shared_workspace(cuda_device):
     rng = np.random.default_rng(2)
     c = _case(rng, 6, 30000, 100, 10, 3)
