@@ -52,8 +52,18 @@ def _device_of(x: torch.Tensor, name: str) -> int:
     return x.get_device()
 
 
-def _stream_of(device: int, stream) -> int:
-    return torch._C._cuda_getCurrentRawStream(device) if stream is None else int(stream.cuda_stream)
+def _stream_of(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _on(stream, device: int):
+    """Makes `stream` (None: the current one) and its device current, so that the memory allocated for a result
+    belongs to the stream that writes it."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device_index != device:
+        raise ValueError(f"the stream is cuda:{stream.device_index}'s, the tensors are on cuda:{device}")
+    return torch.cuda.stream(stream)
 
 
 def add_rms_norm(x: torch.Tensor, w1: torch.Tensor | None = None, eps: float = 1e-6, *,
@@ -66,10 +76,10 @@ def add_rms_norm(x: torch.Tensor, w1: torch.Tensor | None = None, eps: float = 1
     it is stored.  `w1` is 1 + w in f32.  `out_dtype` (x's type by default): bf16, f32, or float8_e4m3fn with one
     f32 scale per row (out * scale is the value).  Returns (out, scales), scales None unless out is e4m3."""
     dev = _device_of(x, "x")
-    if dev != _current_device():
-        with torch.cuda.device(dev):
+    if stream is not None or dev != _current_device():
+        with _on(stream, dev):
             return add_rms_norm(x, w1, eps, residual=residual, sum_out=sum_out, out=out, out_dtype=out_dtype,
-                                scales=scales, stream=stream)
+                                scales=scales)
     xc, xs = _rows(x, "x", _FLOATS, dev)
     shape = x.shape
     n, hidden = shape
@@ -105,7 +115,7 @@ def add_rms_norm(x: torch.Tensor, w1: torch.Tensor | None = None, eps: float = 1
         raise ValueError("scales go with an e4m3 output only")
     if n:
         st = L.lib().mtn_add_rms_norm(x.data_ptr(), xc, xs, rp, rs, sp, ss, rc, w1p, eps, n, hidden, out.data_ptr(), oc,
-                                      os_, scp, _stream_of(dev, stream))
+                                      os_, scp, _stream_of(dev))
         if st:
             L.check(st)
     return out, scales
@@ -123,7 +133,6 @@ class W4Weight:
         self.n, self.k, self.group = n, k, group
         self.packed = torch.empty(nb, dtype=torch.uint8, device=device)
         self.scales = torch.empty(ns // 2, dtype=torch.bfloat16, device=device)
-        self.packed_ptr, self.scales_ptr = self.packed.data_ptr(), self.scales.data_ptr()
 
     @property
     def device(self) -> torch.device:
@@ -134,10 +143,10 @@ class W4Weight:
         """Quantise bf16 / f32 weights [n, k]: per group scale = bf16(max|w| / 7), code = round(w / scale)."""
         dev = _device_of(weight, "weight")
         code, row = _rows(weight, "weight", _FLOATS, dev)
-        w = cls(*weight.shape, group, weight.device)
-        with torch.cuda.device(dev):
+        with _on(stream, dev):
+            w = cls(*weight.shape, group, weight.device)
             L.check(L.lib().mtn_w4_quantize(weight.data_ptr(), code, row, w.n, w.k, group, w.packed.data_ptr(),
-                                            w.scales.data_ptr(), _stream_of(dev, stream)))
+                                            w.scales.data_ptr(), _stream_of(dev)))
         return w
 
     @classmethod
@@ -146,26 +155,26 @@ class W4Weight:
         dev = _device_of(codes, "codes")
         _, code_row = _rows(codes, "codes", {torch.int8: 0}, dev)
         _, scale_row = _rows(scales, "scales", {torch.bfloat16: 0}, dev)
-        w = cls(*codes.shape, group, codes.device)
-        if scales.shape != (w.n, -(-w.k // group)):
-            raise ValueError("scales must be [n, ceil(k / group)]")
-        with torch.cuda.device(dev):
+        with _on(stream, dev):
+            w = cls(*codes.shape, group, codes.device)
+            if scales.shape != (w.n, -(-w.k // group)):
+                raise ValueError("scales must be [n, ceil(k / group)]")
             L.check(L.lib().mtn_w4_pack(codes.data_ptr(), code_row, scales.data_ptr(), scale_row, w.n, w.k, group,
-                                        w.packed.data_ptr(), w.scales.data_ptr(), _stream_of(dev, stream)))
+                                        w.packed.data_ptr(), w.scales.data_ptr(), _stream_of(dev)))
         return w
 
     def dequantize(self, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
                    stream=None) -> torch.Tensor:
         """The values code * scale, row-major [n, k] in f32 (exact) or bf16."""
         dev = self.packed.get_device()
-        if out is None:
-            out = torch.empty((self.n, self.k), dtype=dtype, device=self.device)
-        code, row = _rows(out, "out", _FLOATS, dev)
-        if out.shape != (self.n, self.k):
-            raise ValueError("out must be [n, k]")
-        with torch.cuda.device(dev):
+        with _on(stream, dev):
+            if out is None:
+                out = torch.empty((self.n, self.k), dtype=dtype, device=self.device)
+            code, row = _rows(out, "out", _FLOATS, dev)
+            if out.shape != (self.n, self.k):
+                raise ValueError("out must be [n, k]")
             L.check(L.lib().mtn_w4_dequantize(self.packed.data_ptr(), self.scales.data_ptr(), self.n, self.k, self.group,
-                                              out.data_ptr(), code, row, _stream_of(dev, stream)))
+                                              out.data_ptr(), code, row, _stream_of(dev)))
         return out
 
 
@@ -177,9 +186,9 @@ def w4_matvec(x: torch.Tensor, weight: W4Weight, *, x_scales: torch.Tensor | Non
     defaults to x's type, or bf16 for e4m3.  Meant for the few rows of a decode step: the weights are read once
     per 16 rows; for a prompt's many rows dequantise and use a matrix product."""
     dev = _device_of(x, "x")
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return w4_matvec(x, weight, x_scales=x_scales, out=out, out_dtype=out_dtype, stream=stream)
+    if stream is not None or dev != _current_device():
+        with _on(stream, dev):
+            return w4_matvec(x, weight, x_scales=x_scales, out=out, out_dtype=out_dtype)
     xc, xs = _rows(x, "x", _CODES, dev)
     m, k = x.shape
     if k != weight.k:
@@ -198,8 +207,8 @@ def w4_matvec(x: torch.Tensor, weight: W4Weight, *, x_scales: torch.Tensor | Non
     if weight.packed.get_device() != dev:
         raise ValueError(f"the weight is on {weight.device}, x on {x.device}")
     if m:
-        st = L.lib().mtn_w4_matvec(x.data_ptr(), xc, xs, xsp, m, weight.packed_ptr, weight.scales_ptr, weight.n, k,
-                                   weight.group, out.data_ptr(), oc, os_, _stream_of(dev, stream))
+        st = L.lib().mtn_w4_matvec(x.data_ptr(), xc, xs, xsp, m, weight.packed.data_ptr(), weight.scales.data_ptr(),
+                                   weight.n, k, weight.group, out.data_ptr(), oc, os_, _stream_of(dev))
         if st:
             L.check(st)
     return out

@@ -419,7 +419,6 @@ class LogitsRules:
         self.device_index = None if self.device is None else self.device.index
         self._scratch = (0, 0)  # (rows, bytes) last asked for
 
-
     def scratch_bytes(self, n_rows: int) -> int:
         """Bytes of scratch that mtn_process_logits needs for these lists."""
         if self._scratch[0] != n_rows:
@@ -447,9 +446,14 @@ def process_logits(logits: torch.Tensor, rules: LogitsRules, out: torch.Tensor |
     if not logits.is_cuda:
         raise ValueError("expected a CUDA tensor (there is no CPU implementation)")
     dev = logits.get_device()
+    if stream is not None:
+        if stream.device_index != dev:
+            raise ValueError(f"the stream is cuda:{stream.device_index}'s, the logits are on cuda:{dev}")
+        with torch.cuda.stream(stream):  # the memory that is allocated here belongs to the launch's stream
+            return process_logits(logits, rules, out, tokens, greedy, workspace)
     if dev != _current_device():
         with torch.cuda.device(dev):
-            return process_logits(logits, rules, out, tokens, greedy, workspace, stream)
+            return process_logits(logits, rules, out, tokens, greedy, workspace)
     shape = logits.shape
     n, vocab = shape
     row, unit = logits.stride()
@@ -482,16 +486,11 @@ def process_logits(logits: torch.Tensor, rules: LogitsRules, out: torch.Tensor |
         ws, nws = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     if n == 0:
         return out, tokens
-    scratch, nscratch = None, rules.scratch_bytes(n)
-    if nscratch:
-        if stream is None:
-            scratch = torch.empty(nscratch, dtype=torch.uint8, device=logits.device)
-        else:
-            with torch.cuda.stream(stream):  # the memory belongs to the launch's stream
-                scratch = torch.empty(nscratch, dtype=torch.uint8, device=logits.device)
+    nscratch = rules.scratch_bytes(n)
+    scratch = torch.empty(nscratch, dtype=torch.uint8, device=logits.device) if nscratch else None
     st = L.lib().mtn_process_logits(logits.data_ptr(), code, row, n, vocab, rules._ref, out.data_ptr(), out_row, tp, ws,
                                     nws or 0, None if scratch is None else scratch.data_ptr(), nscratch,
-                                    torch._C._cuda_getCurrentRawStream(dev) if stream is None else int(stream.cuda_stream))
+                                    torch._C._cuda_getCurrentRawStream(dev))
     if st:
         L.check(st)
     return out, tokens

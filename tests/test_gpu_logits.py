@@ -260,6 +260,23 @@ def test_streams_replay_and_shared_workspace(cuda_device):
     assert torch.equal(out, want) and torch.equal(tok, wt)
 
 
+def test_a_workspace_made_for_the_call_is_zeroed_on_its_stream(cuda_device):
+    x = torch.randn(8, 5000, device="cuda")
+    rules = paged.LogitsRules(mask=torch.full((8, 157), -1, dtype=torch.int32, device="cuda"))
+    want = paged.argmax_rows(x)
+    s = torch.cuda.Stream()
+    dirty = [torch.full((512,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    with torch.cuda.stream(s):
+        dirty += [torch.full((512,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    del dirty
+    torch.cuda._sleep(20_000_000)  # the current stream is busy: nothing of the call waits for it
+    out, tokens = paged.process_logits(x, rules, greedy=True, stream=s)
+    s.synchronize()
+    with torch.cuda.stream(s):
+        assert torch.equal(tokens, want) and torch.equal(out, x)
+
+
 def test_wrapper_refuses(cuda_device):
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     f32 = lambda *v: torch.tensor(v, dtype=torch.float32, device="cuda")  # noqa: E731

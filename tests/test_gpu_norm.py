@@ -134,6 +134,25 @@ def test_other_stream_and_captured_replay(cuda_device):
     assert torch.equal(out.view(torch.uint8), want.view(torch.uint8)) and torch.equal(sco, wsc)
 
 
+def test_results_on_another_stream_are_not_written_by_work_still_queued(cuda_device):
+    # memory freed with a fill still queued on the current stream must not become a result on another one
+    x, _, w1 = _inputs(64, 1024, F32, None, 5)
+    want = dense.add_rms_norm(x, w1)[0]
+    w = dense.W4Weight.from_float(torch.randn(1024, 1024, device="cuda"), 128)
+    values, y = w.dequantize(), dense.w4_matvec(x, w)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for call, ref in ((lambda: dense.add_rms_norm(x, w1, stream=s)[0], want), (lambda: w.dequantize(stream=s), values),
+                      (lambda: dense.w4_matvec(x, w, stream=s), y)):
+        freed = torch.empty_like(ref)
+        torch.cuda._sleep(20_000_000)
+        freed.fill_(7.0)
+        del freed
+        got = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, ref)
+
+
 def test_wrapper_refuses(cuda_device):
     x = torch.zeros(4, 64, device="cuda")
     bad = [dict(w1=torch.ones(63, device="cuda")), dict(w1=torch.ones(64, device="cuda", dtype=BF)),
