@@ -470,13 +470,12 @@ class Engine:
             raise ValueError("prompt must be a list of token ids of the vocabulary")
         if not rules.repetition > 0 or not np.isfinite([rules.repetition, rules.presence, rules.frequency]).all():
             raise ValueError("repetition must be positive, and the penalties finite")
-        if any(not 0 <= t < vocab for t in rules.bias) or np.isnan(list(rules.bias.values())).any():
-            raise ValueError("bias: token ids of the vocabulary with values that are numbers")
+        if any(not 0 <= t < vocab for t in rules.bias) or not all(v < np.inf for v in rules.bias.values()):
+            raise ValueError("bias: token ids of the vocabulary with values that are numbers below infinity")
         self._rules[int(req_id)] = (ids.astype(np.int32), rules)
 
-    def _apply_rules(self, b, logits: torch.Tensor, greedy: bool) -> torch.Tensor | None:
-        """The batch's rules on its logits, in place; the greedy tokens if asked for.  Rows without rules pass as
-        they are."""
+    def _apply_rules(self, b, logits: torch.Tensor) -> torch.Tensor:
+        """The batch's rules on its logits, in place; the greedy tokens.  Rows without rules pass as they are."""
         n, vocab = logits.shape
         mine = [self._rules.get(int(r)) for r in b.req_ids]
         out = [self.sched.request_output(int(r)) if m else [] for r, m in zip(b.req_ids, mine)]
@@ -513,10 +512,31 @@ class Engine:
                 masks.append(np.packbits(bits, bitorder="little").view(np.int32))
         if masks:
             kw["mask"], kw["mask_rows"] = up(np.stack(masks), np.int32), up(rows, np.int32)
-        if greedy and (self._rules_ws is None or self._rules_ws.numel() < 16 * n):
+        if self._rules_ws is None or self._rules_ws.numel() < 16 * n:
             self._rules_ws = paged.logits_workspace(n, dev)
-        return paged.process_logits(logits, paged.LogitsRules(**kw), out=logits, greedy=greedy,
+        return paged.process_logits(logits, paged.LogitsRules(**kw), out=logits, greedy=True,
                                     workspace=self._rules_ws)[1]
+
+    def _sample(self, logits: torch.Tensor, temperatures: np.ndarray, picked: torch.Tensor | None, b) -> torch.Tensor:
+        """mtn_sample_rows; `picked`: the greedy tokens where rules were applied.
+
+        The sampler takes exp(x / t) as it stands (scheduler.rs:201-222) and, at a random number of 0 or where no
+        running sum reaches it, a token of probability 0.  Rows with rules must not depend on that: their logits
+        are shifted by their maximum where the exponentials' sum could leave f32's range (a large bias, or a mask
+        that leaves only small ones), and a token that the rules forbid gives way to the greedy one."""
+        nb = L.lib().mtn_sample_rows_workspace_bytes(*logits.shape)
+        if self._sample_ws is None or self._sample_ws.numel() < nb:
+            self._sample_ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
+        temps = torch.from_numpy(temperatures).to(logits.device)
+        if picked is None:
+            return paged.sample_rows(logits, temps, workspace=self._sample_ws)
+        ruled = torch.tensor([int(r) in self._rules for r in b.req_ids], device=logits.device) & (temps > 0)
+        top = logits.gather(1, picked.long()[:, None])[:, 0]
+        far = ((top / temps).abs() > 88.0 - np.log(logits.shape[1])) & torch.isfinite(top)  # ln of f32's maximum: 88.7
+        logits.sub_(torch.where(ruled & far, top, 0.0)[:, None])
+        tokens = paged.sample_rows(logits, temps, workspace=self._sample_ws)
+        lost = logits.gather(1, tokens.long()[:, None])[:, 0].isneginf() | ~torch.isfinite(top)
+        return torch.where(ruled & lost, picked, tokens)
 
     def _drop_rules(self, b) -> None:
         """Forget the rules of requests that have ended."""
@@ -534,15 +554,11 @@ class Engine:
             picked = None
             if any(int(r) in self._rules for r in b.req_ids):
                 try:
-                    picked = self._apply_rules(b, logits, not hot)
+                    picked = self._apply_rules(b, logits)
                 except Exception as e:  # a request's allowed() is the caller's code
                     raise RuntimeError("the batch's token rules could not be applied") from e
             if hot:
-                nb = L.lib().mtn_sample_rows_workspace_bytes(*logits.shape)
-                if self._sample_ws is None or self._sample_ws.numel() < nb:
-                    self._sample_ws = torch.empty(nb, dtype=torch.uint8, device=logits.device)
-                temps = torch.from_numpy(b.temperatures).to(logits.device)
-                tokens = paged.sample_rows(logits, temps, workspace=self._sample_ws).cpu().numpy().astype(np.uint32)
+                tokens = self._sample(logits, b.temperatures, picked, b).cpu().numpy().astype(np.uint32)
             else:
                 tokens = (paged.argmax_rows(logits) if picked is None else picked).cpu().numpy().astype(np.uint32)
             code, detail = paged.device_error(self.model.dev.index or 0)

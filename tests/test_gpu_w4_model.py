@@ -253,3 +253,37 @@ def test_temperature_rows_sample_the_processed_logits(cuda_device):
     for rid in range(3):
         out = sched.request_output(rid)
         assert len(out) == 6 and set(out) <= {17, 400}
+
+
+def _sampled(cfg, model, rules, temperature, steps=4):
+    sched = host.Scheduler(64, 16, eos_token_ids=(cfg.vocab,))
+    eng = M.Engine(model, sched, cuda_graphs=False)
+    sched.add_request(0, np.arange(7, dtype=np.uint32), temperature=temperature, max_new_tokens=steps)
+    if rules is not None:
+        eng.set_rules(0, np.arange(7), rules)
+    eng.run()
+    return sched.request_output(0)
+
+
+def test_sampling_with_rules_keeps_to_them(cuda_device, monkeypatch):
+    cfg = R.QwenShape(hidden=256, layers=1, hq=14, hkv=2, head_dim=64, inter=512, vocab=1000)
+    model = M.QwenPagedModel(shape_of(cfg), R.random_weights(cfg, seed=1), 64, 16)
+    # neutral rules change nothing
+    assert _sampled(cfg, model, M.TokenRules(), 0.9) == _sampled(cfg, model, None, 0.9)
+    # exp(x / t) overflows f32 with the bias, and vanishes with the mask and the negative one
+    assert _sampled(cfg, model, M.TokenRules(bias={33: 100.0}), 0.5) == [33] * 4
+    only = np.zeros(cfg.vocab, bool)
+    only[[17, 400]] = True
+    out = _sampled(cfg, model, M.TokenRules(bias={17: -200.0, 400: -200.0}, allowed=lambda o: only), 0.5)
+    assert set(out) <= {17, 400}
+    # nothing allowed: the greedy token of such a row
+    assert _sampled(cfg, model, M.TokenRules(allowed=lambda o: np.zeros(cfg.vocab, bool)), 0.9) == [0] * 4
+    # a random number of 0, or no running sum that reaches it: the sampler's first and last tokens
+    for forbidden in (0, cfg.vocab - 1):
+        monkeypatch.setattr(M.paged, "sample_rows", lambda x, t, workspace=None, f=forbidden: torch.full(
+            (x.shape[0],), f, dtype=torch.int32, device=x.device))
+        out = _sampled(cfg, model, M.TokenRules(allowed=lambda o: only), 0.9)
+        assert len(out) == 4 and set(out) <= {17, 400}
+    with pytest.raises(ValueError):
+        M.Engine(model, host.Scheduler(64, 16, eos_token_ids=(cfg.vocab,))).set_rules(
+            0, [1], M.TokenRules(bias={1: float("inf")}))
