@@ -238,8 +238,7 @@ MTN_API int mtn_add_rms_norm(const void* x, int32_t x_dtype, int64_t x_stride, c
  * bf16 or f32; out must not overlap x.  Every call reads the weights at least
  * once per 16 rows.  mtn_add_rms_norm and mtn_w4_matvec are launched with
  * programmatic dependent launch: they may begin while the kernel before them
- * finishes, but wait for it before they read or write anything (a matvec first
- * asks for some of its weights in L2). */
+ * finishes, but wait for it before they read or write anything. */
 MTN_API size_t mtn_w4_packed_bytes(int64_t n, int64_t k);
 MTN_API size_t mtn_w4_scales_bytes(int64_t n, int64_t k, int32_t group);
 MTN_API int mtn_w4_quantize(const void* weight, int32_t dtype, int64_t stride, int64_t n, int64_t k, int32_t group,

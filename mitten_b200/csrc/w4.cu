@@ -22,6 +22,7 @@
 // along k, then along the rows.  Scales: [row unit][k / G][8] words, word g
 // holding row g's scale in its low half and row g + 8's in its high half.
 #include <algorithm>
+#include <atomic>
 
 #include <cuda_fp8.h>
 
@@ -541,18 +542,10 @@ __global__ void __launch_bounds__(kMvThreads, 1) w4_matvec_kernel(const W4Params
       }
     };
     if (u0 == cu0) {
-      // What the kernel before this one does not write may start early: the
-      // weights on their way into L2.
-      seek();
-      for (int d = 0; d < min(min(kD, n_items), L - ls); ++d)
-#pragma unroll
-        for (int r = 0; r < kR; ++r) {
-          const uint4* w = wp[r] + d * 64;
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(w));
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(w + 32));
-        }
       pdl_enter();
-      // x before the weights: behind them it would wait for all their bytes
+      // x before the weights: behind them it would wait for all their bytes.  (Asking for the weights in L2
+      // before the wait above did as much harm as good: with add_rms_norm before it 8 x 18944 x 3584 took
+      // 13.9 us against 14.3 for both, 1 x 18944 x 3584 11.6 against 11.2.)
       if (direct) {
         copy_rows(p, plan, smem_u32(xs), m0, mt, k0, L * kKPad);
         cp_async_commit();
@@ -739,7 +732,7 @@ MvKernel mv_kernel(int parts, int nt, int r, int group) {
 // Clusters of `size` CTAs that the device holds at once (one CTA per SM).
 int max_clusters(int size) {
   constexpr int kDevices = 64;
-  static int cached[kDevices][4] = {};
+  static std::atomic<int> cached[kDevices][4];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return std::max(1, 128 / size);
   const int slot = size == 1 ? 0 : size == 2 ? 1 : size == 4 ? 2 : 3;
