@@ -96,6 +96,76 @@ def test_general_values(cuda_device, n, k, group, xd, od):
         assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() / tol).max()
 
 
+# More than 16 rows of whole steps of k and 2^22 weights or more go to the tcgen05 products: slices of k over 1 to 8
+# CTAs, tiles that are partly there, a second pass of rows, groups of every size, each of the row types.
+@pytest.mark.parametrize("n,k", [(32768, 128), (3584, 1280), (2056, 2048), (18950, 256), (128, 32768), (37888, 384),
+                                 (64, 65536), (70, 65536), (4099, 1024)])
+@pytest.mark.parametrize("group,xd", [(32, BF), (64, E4), (128, F32), (128, BF), (32, F32), (64, BF), (32, E4)])
+def test_more_than_sixteen_rows(cuda_device, n, k, group, xd):
+    g = _gen(n + k + group)
+    codes = _codes(n, k, g)
+    scales = (0.01 * (0.2 + torch.rand(n, k // group, generator=g, device="cuda"))).to(BF)
+    w = dense.W4Weight.from_codes(codes, scales, group)
+    val = _values(codes, scales, group)
+    ones = dense.W4Weight.from_codes(codes, torch.full_like(scales, 2.0 ** -5), group)
+    for m in (17, 31, 32, 33, 70):
+        big = torch.randn(m, k + 16, generator=g, device="cuda")
+        xs = big.abs().amax(1) / 448.0 if xd == E4 else None
+        x = (big if xs is None else big / xs[:, None]).to(xd)[:, 16:]  # rows with a stride
+        out = torch.full((m + 1, n + 3), 7.0, device="cuda")
+        dense.w4_matvec(x, w, x_scales=xs, out=out[:m, :n])
+        assert (out[m] == 7).all() and (out[:, n:] == 7).all()
+        xv = x.double() if xs is None else x.double() * xs.double()[:, None]
+        want, mag = xv @ val.T, xv.abs() @ val.abs().T
+        tol = 4 * (k / 16 + 64) * U * mag
+        tol = tol + U * (want.abs() + tol)
+        got = out[:m, :n].double()
+        assert ((got - want).abs() <= tol).all(), (m, ((got - want).abs() / tol).max())
+        again = dense.w4_matvec(x, w, x_scales=xs, out_dtype=F32)
+        assert torch.equal(again, out[:m, :n])
+        xi = torch.randint(-2, 3, (m, k), generator=g, device="cuda").float()  # sums of these are exact
+        one = None if xd != E4 else torch.ones(m, device="cuda")
+        got = dense.w4_matvec(xi.to(xd), ones, x_scales=one, out_dtype=F32)
+        assert torch.equal(got.double(), (xi.double() @ codes.double().T) * 2.0 ** -5)
+    assert paged.device_error(0) == (0, 0)
+
+
+def test_more_than_sixteen_rows_with_values_that_are_none(cuda_device):
+    g = _gen(3)
+    codes, scales = _codes(4096, 1024, g), torch.full((4096, 8), 0.5, device="cuda", dtype=BF)
+    scales[5, 2], scales[300, 0] = float("nan"), float("inf")
+    codes[:, 700] = 3
+    w = dense.W4Weight.from_codes(codes, scales, 128)
+    x = torch.randn(20, 1024, generator=g, device="cuda").to(BF)
+    want = dense.w4_matvec(x, w)
+    x[3, 700], x[9, 700] = float("nan"), float("inf")
+    got = dense.w4_matvec(x, w)
+    other = [r for r in range(20) if r not in (3, 9)]
+    assert torch.equal(got[other].nan_to_num(7, 8, 9), want[other].nan_to_num(7, 8, 9))
+    assert got[:, 5].isnan().all() and got[3].isnan().all()
+    fine = [c for c in range(4096) if c not in (5, 300)]
+    assert (got[9][fine] == float("inf")).all() and not got[other][:, fine].isnan().any()
+    # captured and replayed, behind and before a norm
+    h, out = torch.empty_like(x[:, :1024]), torch.empty(20, 4096, device="cuda", dtype=BF)
+    x = torch.randn(20, 1024, generator=g, device="cuda").to(BF)
+    scales.fill_(0.5)
+    w = dense.W4Weight.from_codes(codes, scales, 128)
+    graph = torch.cuda.CUDAGraph()
+    dense.add_rms_norm(x, out=h)
+    want = dense.w4_matvec(h, w)
+    want2 = dense.add_rms_norm(want)[0]
+    h.zero_()
+    res = torch.empty_like(want2)
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            dense.add_rms_norm(x, out=h)
+            dense.w4_matvec(h, w, out=out)
+            dense.add_rms_norm(out, out=res)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(res, want2)
+
+
 def test_same_result_every_time_and_for_rows_alone(cuda_device):
     g = _gen(9)
     codes, scales = _codes(1000, 3584, g), torch.rand(1000, 28, generator=g, device="cuda").to(BF)
