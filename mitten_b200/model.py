@@ -70,11 +70,10 @@ GEMMA_2B = DecoderShape(hidden=2048, layers=18, hq=8, hkv=1, head_dim=256, inter
                         gated_q=False, qk_norm=False, phantom=False, mlp="geglu")
 
 
-# Rows up to which the 4-bit product (which reads the weights once per 16 or 32 rows) beats dequantising a matrix and
-# multiplying: 18944 x 3584 takes 41 and 62 us with 64 bf16 rows, 60 and 62 with 96, 3584 x 18944 47 and 70, 69 and 70,
-# 3584 x 3584 17 and 15, 26 and 15; in f32 255 and 548 us with 192 rows, 367 and 595 with 256, 9728 x 896 103 and 87
-# with 192.
-W4_MATVEC_ROWS = {torch.bfloat16: 64, torch.float32: 192}
+# Rows up to which the 4-bit matrix-vector product (which reads the weights once per 16 rows) beats dequantising
+# a matrix and multiplying: 18944 x 3584 takes 42 and 56 us with 48 bf16 rows, 55 and 61 with 64, 3584 x 18944 74
+# and 69 with 64; in f32 273 and 333 us with 128 rows, 545 and 592 with 256, 9728 x 896 76 and 77 with 128.
+W4_MATVEC_ROWS = {torch.bfloat16: 48, torch.float32: 128}
 
 
 def _rms(x: torch.Tensor, w1: torch.Tensor, eps: float) -> torch.Tensor:
