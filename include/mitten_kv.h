@@ -236,7 +236,7 @@ MTN_API int mtn_add_rms_norm(const void* x, int32_t x_dtype, int64_t x_stride, c
  * mtn_w4_matvec: x bf16, f32, or e4m3 with x_scales (what mtn_add_rms_norm
  * writes; NULL for the other types), n_rows up to 65535; sums in f32, out
  * bf16 or f32; out must not overlap x.  Every call reads the weights at least
- * once per 32 rows.  mtn_add_rms_norm and mtn_w4_matvec are launched with
+ * once per 16 rows.  mtn_add_rms_norm and mtn_w4_matvec are launched with
  * programmatic dependent launch: they may begin while the kernel before them
  * finishes, but wait for it before they read or write anything. */
 MTN_API size_t mtn_w4_packed_bytes(int64_t n, int64_t k);

@@ -27,7 +27,6 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
-#include "tc.cuh"
 
 namespace mtn {
 namespace {
@@ -819,463 +818,6 @@ MvPlan mv_plan(int64_t m, int64_t n, int64_t k, int group, int parts) {
   return pl;
 }
 
-// ------------------------------------------------------ 17 rows and more
-//
-// There mma.sync is what bounds the kernel above, and it reads the weights
-// once per 16 rows.  Here the products are tcgen05.mma: 128 weight rows as the
-// A operand in tensor memory, 32 x rows as B in shared memory, a group's sums
-// in tensor memory.  A step is 128 k of a tile of 8 row units; the roles of a
-// CTA's warps:
-//   0-7    unpack: their lanes' weights through a cp.async ring, to bf16
-//          q / 8, to A.  tcgen05.st 16x256b has the layout of the weights'
-//          words: lane 4 g + t holds rows g and g + 8 of a row unit and, of
-//          every 16 k, the pairs 2 t, 2 t + 1.  So a word's first half lands
-//          in one 16 k and its second in the next, and x is stored in that
-//          order of k.  Warps w and w + 4 take alternate steps of row units
-//          2 w, 2 w + 1.
-//   8-11   sums: each group's out of tensor memory, times the group's scale,
-//          added up in f32 registers, a thread per weight row.
-//   12-15  x: rows of a step to bf16 (f32: three parts) in shared memory,
-//          128-byte swizzled; a warp per buffer.
-//   16     issues the products.
-// A cluster of S CTAs takes a contiguous range of row units, each CTA an S-th
-// of k; with S > 1 the CTAs' sums are added in rank order over distributed
-// shared memory after every tile.  Waits have a limit: one that runs out
-// records device error 4, and the kernel ends with undefined results.
-//
-// 32 x 3584 x 3584 takes 8.4 us (18.5 with the kernel above), 32 x 18944 x
-// 3584 21.8 (31.2), 32 x 3584 x 18944 25.0 (36.9), f32 rows 44.6 (68.5).  The
-// thread that waits for a step, issues its products and commits them is the
-// bound, 0.5 to 0.75 us a step; so CTAs of more than two tiles, few weights and
-// up to 16 rows are left to the kernel above (tc_plan).
-constexpr int kTcThreads = 17 * 32;
-constexpr int kTcN = 32;        // x rows of a pass
-constexpr int kTcRows = 8;      // row units of a tile
-constexpr int kTcRing = 5;      // weight steps ahead of an unpacking warp
-constexpr int kTcA = 4;         // buffers of A (64 columns each) and x, a staging warp each
-constexpr int kTcScales = 8;    // scale steps ahead
-constexpr uint32_t kTcCols = 512;
-constexpr int kTcBars = 2 * kTcA + 1;
-
-struct TcPlan {
-  int cluster, clusters, per, extra, tile;
-  int* err;
-};
-
-template <int kParts, int kGroups>
-struct TcSmem {
-  static constexpr int kXBytes = kParts * kTcN * 256;
-  static constexpr int kScaleBytes = 2 * kGroups * 32;
-  static constexpr int kRingOff = kTcA * kXBytes;
-  static constexpr int kScaleOff = kRingOff + 8 * kTcRing * 2048;
-  static constexpr int kPartOff = kScaleOff + 4 * kTcScales * kScaleBytes;
-  static constexpr int kBarOff = kPartOff + kTcN * 128 * 4;
-  static constexpr int kBytes = kBarOff + kTcBars * 8 + 16 + 1024;  // the base is moved to 1024 bytes
-};
-
-// 16 lanes x 32 columns of a row unit's 64 k.
-__device__ __forceinline__ void tmem_st_unit(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(at));
-}
-
-// One lane of a converged warp.
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r;
-}
-
-// D[tmem] (+)= A[tmem] * B[smem], issued by the lane that has `one`, in code that the whole warp runs.
-__device__ __forceinline__ void mma_ts_one(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
-                                           uint32_t one) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
-      : "memory");
-}
-
-__device__ __forceinline__ void commit_one(uint64_t* bar, uint32_t one) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(one)
-      : "memory");
-}
-
-// 8 bytes, asynchronous.
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-
-enum XKind { kXBf16, kXE4m3, kXF32 };
-
-__device__ __forceinline__ void sts8(uint32_t at, uint32_t a, uint32_t b) {
-  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
-}
-
-template <XKind kKind, int kGroups>
-__global__ void __launch_bounds__(kTcThreads, 1) w4_rows_kernel(const W4Params p, const TcPlan plan) {
-  constexpr int kParts = kKind == kXF32 ? 3 : 1;
-  using M = TcSmem<kParts, kGroups>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* part = reinterpret_cast<float*>(smem + M::kPartOff);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + M::kBarOff);
-  // full: A (4 warps), x (1) and the sums' columns (4) are ready for a step; done: its products have ended
-  uint64_t *full = bars, *done = full + kTcA, *last = done + kTcA;
-  constexpr int kBufs = kTcN * kGroups > 64 ? 2 : kTcA;  // of 512 columns: 64 each for A, kTcN * kGroups for sums
-  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(bars + kTcBars);
-  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3;
-  const int S = plan.cluster;
-  const int rank = S > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int cl = static_cast<int>(blockIdx.x) / S;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * plan.tile;
-  const int mt = static_cast<int>(min(static_cast<int64_t>(plan.tile), p.m - m0));
-  const int ksteps = static_cast<int>(pad_k(p.k) / kKPad);
-  const int cu0 = cl * plan.per + min(cl, plan.extra), cu1 = cu0 + plan.per + (cl < plan.extra ? 1 : 0);
-  const int s0 = rank * ksteps / S, L = (rank + 1) * ksteps / S - s0;
-  const int tiles = (cu1 - cu0 + kTcRows - 1) / kTcRows, total = tiles * L;
-
-  pdl_enter();
-  if (tid == 0) {
-    for (int i = 0; i < kTcA; ++i) mbar_init(&full[i], 9), mbar_init(&done[i], 1);
-    mbar_init(last, 1);
-    fence_barrier_init();
-  }
-  if (warp == 0) {
-    tc::tmem_alloc(tmem_base, kTcCols);
-    tc::tmem_relinquish();
-  }
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
-  const uint32_t tmem = *tmem_base, one = elect_one();
-  const uint32_t tmem_d = tmem + kBufs * 64;
-  auto wait = [&](uint64_t* bar, int use, int where) {  // use: 0 for a barrier's first completion
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, use & 1, plan.err, where)) != 0;
-  };
-
-  const int set = warp >> 2;  // 0 or 1 of the unpacking warps
-  // rings of steps on their way: an unpacking warp's weights, a summing warp's scales
-  const uint32_t ring = smem_u32(smem + M::kRingOff) + warp * (kTcRing * 2048);
-  const uint32_t srings = smem_u32(smem + M::kScaleOff) + q * (kTcScales * M::kScaleBytes);
-  const int runits = static_cast<int>(row_units(p.n));
-  int slot = 0, lt = 0, ls = 0;  // of the next load: ring slot, tile, step of the slice
-  if (warp < 8 && set == 1 && ++ls == L) ls = 0, ++lt;
-  auto advance = [&](int steps, int slots) {
-    for (int i = 0; i < steps; ++i)
-      if (++ls == L) ls = 0, ++lt;
-    if (++slot == slots) slot = 0;
-  };
-  auto load_weights = [&]() {
-    if (lt < tiles && L > 0) {
-      const uint32_t at = ring + slot * 2048 + lane * 16;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int ru = cu0 + lt * kTcRows + 2 * q + r;
-        if (ru >= cu1) continue;
-        const uint4* src = p.packed + (static_cast<int64_t>(ru) * ksteps + s0 + ls) * 64 + lane;
-        cp_async16(at + r * 1024, src);
-        cp_async16(at + r * 1024 + 512, src + 32);
-      }
-    }
-    cp_async_commit();
-    advance(2, kTcRing);
-  };
-  auto load_scales = [&]() {
-    if (lt < tiles && L > 0 && lane < 4 * kGroups) {
-      const int r = lane / (2 * kGroups), c = lane - r * 2 * kGroups;
-      const int ru = min(cu0 + lt * kTcRows + 2 * q + r, runits - 1);
-      cp_async16(srings + slot * M::kScaleBytes + lane * 16,
-                 reinterpret_cast<const uint4*>(p.scales) + (static_cast<int64_t>(ru) * ksteps + s0 + ls) * (kGroups * 2) + c);
-    }
-    cp_async_commit();
-    advance(1, kTcScales);
-  };
-  if (warp < 8) {
-#pragma unroll 1
-    for (int d = 0; d < kTcRing; ++d) load_weights();
-  } else if (warp < 12) {
-#pragma unroll 1
-    for (int d = 0; d < kTcScales; ++d) load_scales();
-    if (lane < kBufs) tc::mbar_arrive(&full[lane]);  // the sums' columns are free
-  }
-
-  bool ok = true;
-  int mine = warp < 8 ? set : warp < 12 || warp == 16 ? 0 : warp - 12 < kBufs ? warp - 12 : total;  // the role's next step
-  for (int tile = 0; tile < tiles; ++tile) {
-    const int end = (tile + 1) * L;
-    if (warp < 8) {
-      for (; ok && mine < end; mine += 2) {
-        const int i = mine, buf = i % kBufs;
-        cp_async_wait<kTcRing - 1>();
-        ok = wait(&done[buf], i / kBufs + 1, 31);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint32_t at = ring + slot * 2048 + lane * 16;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (cu0 + tile * kTcRows + 2 * q + r >= cu1) continue;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint4 w = lds16(at + r * 1024 + u * 512);
-            const uint32_t v[16] = {code_pair<0>(w.x), code_pair<1>(w.x), code_pair<0>(w.z), code_pair<1>(w.z),
-                                    code_pair<2>(w.x), code_pair<3>(w.x), code_pair<2>(w.z), code_pair<3>(w.z),
-                                    code_pair<0>(w.y), code_pair<1>(w.y), code_pair<0>(w.w), code_pair<1>(w.w),
-                                    code_pair<2>(w.y), code_pair<3>(w.y), code_pair<2>(w.w), code_pair<3>(w.w)};
-            tmem_st_unit(tmem + (static_cast<uint32_t>(q * 32 + r * 16) << 16) + buf * 64 + u * 32, v);
-          }
-        }
-        tc::tmem_st_wait();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&full[buf]);
-        load_weights();
-      }
-    } else if (warp < 12) {
-      float acc[kTcN] = {};
-      for (; ok && mine < end; ++mine) {
-        const int i = mine;
-        cp_async_wait<kTcScales - 1>();
-        __syncwarp();
-        const uint32_t sc = srings + slot * M::kScaleBytes + (lane >> 4) * (kGroups * 32) + (lane & 7) * 4;
-        const int buf = i % kBufs;
-        ok = wait(&done[buf], i / kBufs, 32);
-        if (!ok) break;
-        tc::fence_after_sync();
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const uint32_t s2 = lds4(sc + g * 32);
-          const float s = __uint_as_float(lane & 8 ? s2 & 0xffff0000u : s2 << 16);
-          uint32_t v[kTcN / 16][16];
-#pragma unroll
-          for (int c = 0; c < kTcN / 16; ++c)
-            tmem_ld16(tmem_d + (static_cast<uint32_t>(q * 32) << 16) + (buf * kGroups + g) * kTcN + c * 16, v[c]);
-          tc::tmem_ld_wait();
-          if (g == kGroups - 1) {
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&full[buf]);
-          }
-#pragma unroll
-          for (int c = 0; c < kTcN; ++c) acc[c] = fmaf(__uint_as_float(v[c / 16][c % 16]), s, acc[c]);
-        }
-        __syncwarp();  // every lane has read the scales
-        load_scales();
-      }
-      if (S > 1) {
-#pragma unroll
-        for (int m = 0; m < kTcN; ++m) part[m * 128 + q * 32 + lane] = acc[m];
-      } else {
-        const int64_t row = static_cast<int64_t>(cu0 + tile * kTcRows) * 16 + q * 32 + lane;
-        if (ok && row < p.n && row < static_cast<int64_t>(cu1) * 16) {
-#pragma unroll
-          for (int m = 0; m < kTcN; ++m)
-            if (m < mt) store_out(p, m0 + m, row, acc[m]);
-        }
-      }
-    } else if (warp < 16) {
-      // Chunks of 8 k, 16 to a row: lane l takes chunk l & 15 of every other row.
-      constexpr int kBatch = kParts == 3 ? 4 : 8, kUnits = kTcN / 2 / kBatch;
-      const int c = lane & 15, cc = c & 7, c16 = 4 * (cc >> 2) + ((cc & 3) >> 1), r0 = lane >> 4;
-      uint32_t lo[4], hi[4];  // of rows r0, r0 + 2, r0 + 4, r0 + 6
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const uint32_t at = smem_u32(smem) + (c >> 3) * (kTcN * 128) + (cc & 1) * 8 + (r0 + 2 * b) * 128;
-        lo[b] = at + ((c16 ^ (r0 + 2 * b)) << 4);
-        hi[b] = at + (((c16 + 2) ^ (r0 + 2 * b)) << 4);
-      }
-      auto store = [&](const Raw8& v, uint32_t off, int b) {
-        const uint32_t* w = v.w;
-        if constexpr (kKind == kXBf16) {
-          sts8(lo[b & 3] + off, w[0], w[1]);
-          sts8(hi[b & 3] + off, w[2], w[3]);
-        } else if constexpr (kKind == kXE4m3) {
-          sts8(lo[b & 3] + off, e4m3_pair(w[0], 0), e4m3_pair(w[0], 1));
-          sts8(hi[b & 3] + off, e4m3_pair(w[1], 0), e4m3_pair(w[1], 1));
-        } else {
-          uint16_t h[8][3];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) split3(__uint_as_float(w[j]), h[j]);
-#pragma unroll
-          for (int z = 0; z < 3; ++z) {
-            uint32_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = h[2 * j][z] | static_cast<uint32_t>(h[2 * j + 1][z]) << 16;
-            sts8(lo[b & 3] + off + z * (kTcN * 256), o[0], o[1]);
-            sts8(hi[b & 3] + off + z * (kTcN * 256), o[2], o[3]);
-          }
-        }
-      };
-      auto give = [&](int stage) {
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&full[stage]);
-      };
-      const int64_t row_at = (m0 + r0) * p.x_stride;
-      constexpr int kSize = kKind == kXF32 ? 4 : kKind == kXBf16 ? 2 : 1;
-      const uint8_t* x0 = static_cast<const uint8_t*>(p.x) + (row_at + static_cast<int64_t>(s0) * kKPad + c * 8) * kSize;
-      const int64_t two = 2 * p.x_stride * kSize;
-      for (; ok && mine < end; mine += kBufs) {
-        const int stage = mine % kBufs;
-        const uint32_t off = stage * M::kXBytes;
-        const uint8_t* at = x0 + static_cast<int64_t>(mine - tile * L) * (kKPad * kSize);
-        if constexpr (kKind == kXBf16) {
-          ok = wait(&done[stage], mine / kBufs + 1, 33);
-          if (!ok) break;
-#pragma unroll
-          for (int b = 0; b < kTcN / 2; ++b) {
-            if (r0 + 2 * b < mt) {
-              cp_async8(lo[b & 3] + off + (b >> 2) * 1024, at);
-              cp_async8(hi[b & 3] + off + (b >> 2) * 1024, at + 8);
-            }
-            at += two;
-          }
-          cp_async_commit();
-          cp_async_wait<0>();
-        } else {
-#pragma unroll 1
-          for (int u = 0; u < kUnits; ++u) {
-            Raw8 v[kBatch];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-              if (r0 + 2 * (kBatch * u + b) < mt) {
-                if constexpr (kKind == kXE4m3) {
-                  const uint2 d = *reinterpret_cast<const uint2*>(at);
-                  v[b].w[0] = d.x, v[b].w[1] = d.y;
-                } else {
-                  const uint4 d = *reinterpret_cast<const uint4*>(at), e = *reinterpret_cast<const uint4*>(at + 16);
-                  v[b].w[0] = d.x, v[b].w[1] = d.y, v[b].w[2] = d.z, v[b].w[3] = d.w;
-                  v[b].w[4] = e.x, v[b].w[5] = e.y, v[b].w[6] = e.z, v[b].w[7] = e.w;
-                }
-              }
-              at += two;
-            }
-            if (u == 0) {
-              ok = wait(&done[stage], mine / kBufs + 1, 33);
-              if (!ok) break;
-            }
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) store(v[b], off + (kBatch * u + (b & ~3)) * 256, b);
-          }
-          if (!ok) break;
-        }
-        give(stage);
-      }
-    } else {
-      constexpr uint32_t id = tc::idesc_bf16(128, kTcN, false);
-      constexpr int kPer = 8 / kGroups;  // 16 k each
-      const uint64_t x0 = tc::sdesc_sw128(smem_u32(smem), 16, 1024);
-      for (; ok && mine < end; ++mine) {
-        const int i = mine, buf = i % kBufs;
-        ok = wait(&full[buf], i / kBufs, 34);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint64_t b0 = x0 + buf * (M::kXBytes >> 4);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-          for (int z = 0; z < kParts; ++z)
-            mma_ts_one(tmem_d + (buf * kGroups + kk / kPer) * kTcN, tmem + buf * 64 + kk * 8,
-                       b0 + ((z * (kTcN * 256) + (kk >> 2) * (kTcN * 128) + (kk & 3) * 32) >> 4), id,
-                       kk % kPer > 0 || z > 0 ? 1u : 0u, one);
-        commit_one(&done[buf], one);
-      }
-    }
-    if (S > 1) {
-      cluster_sync();
-      const uint32_t part_at = smem_u32(part);
-      for (int i = rank * kTcThreads + tid; i < mt * 128; i += S * kTcThreads) {
-        const int64_t row = static_cast<int64_t>(cu0 + tile * kTcRows) * 16 + (i & 127);
-        if (row >= p.n || row >= static_cast<int64_t>(cu1) * 16) continue;
-        float v[8];
-#pragma unroll
-        for (int rk = 0; rk < 8; ++rk)
-          if (rk < S) v[rk] = ld_cluster(part_at + i * 4, rk);
-        float sum = 0.0f;
-#pragma unroll
-        for (int rk = 0; rk < 8; ++rk)
-          if (rk < S) sum += v[rk];
-        store_out(p, m0 + (i >> 7), row, sum);
-      }
-      cluster_sync();
-    }
-  }
-  cp_async_wait<0>();
-  if (warp == 16) {  // every product has ended before the tensor memory goes back
-    commit_one(last, one);
-    mbar_wait_bounded(last, 0, plan.err, 37);
-  }
-  __syncwarp();
-  tc::fence_before_sync();
-  __syncthreads();
-  if (warp == 0) {
-    tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, kTcCols);
-  }
-}
-
-using TcKernel = void (*)(const W4Params, const TcPlan);
-
-template <XKind kKind>
-TcKernel tc_kernel(int group, int& smem) {
-  constexpr int kParts = kKind == kXF32 ? 3 : 1;
-  switch (group) {
-    case 32: smem = TcSmem<kParts, 4>::kBytes; return w4_rows_kernel<kKind, 4>;
-    case 64: smem = TcSmem<kParts, 2>::kBytes; return w4_rows_kernel<kKind, 2>;
-    default: smem = TcSmem<kParts, 1>::kBytes; return w4_rows_kernel<kKind, 1>;
-  }
-}
-
-// Whether the products go to w4_rows_kernel, and their split: that whose CTAs
-// take the least time, in 16 x 128 units unpacked: a step's latency counts
-// kTcStep of them, the join of a tile kTcJoin.  Left to w4_matvec_kernel: up
-// to 16 rows (16 x 18944 x 3584: 17.4 us there, 16.4 here; 16 x 152064 x 3584:
-// 80.7 and 111), few weights (32 x 512 x 3584: 5.6 and 6.5; 32 x 4864 x 896:
-// 13.9 and 9.9), more than kTcTiles tiles a CTA (32 x 37888 x 3584: 47.8 and
-// 39.6; 32 x 152064 x 896: 48.4 and 65.1), rows that end inside a step or
-// allow no vector loads.
-constexpr int kTcStep = 12, kTcJoin = 60, kTcTiles = 2;
-constexpr int64_t kTcWeights = 1 << 22;
-
-bool tc_plan(int64_t m, int64_t n, int64_t k, bool x_vec, TcPlan& pl) {
-  if (m <= 16 || n * k < kTcWeights || k % kKPad != 0 || !x_vec) return false;
-  const int ksteps = static_cast<int>(k / kKPad);
-  const int64_t units = row_units(n);
-  pl.tile = kTcN;
-  int64_t best = INT64_MAX, most = 0;
-  for (int s = 1; s <= 8; s *= 2) {
-    const int64_t c = std::min<int64_t>(units, max_clusters(s));
-    const int64_t per = (units + c - 1) / c, tiles = (per + kTcRows - 1) / kTcRows;
-    if (s == 1) most = tiles;
-    const int64_t cost = (per + tiles * kTcStep) * ((ksteps + s - 1) / s) + (s == 1 ? 0 : tiles * kTcJoin);
-    if (cost < best) {
-      best = cost;
-      pl.cluster = s;
-      pl.clusters = static_cast<int>(c);
-      pl.per = static_cast<int>(units / c);
-      pl.extra = static_cast<int>(units % c);
-    }
-  }
-  return most <= kTcTiles;
-}
-
 int check_sizes(const char* who, int64_t n, int64_t k, int32_t group) {
   MTN_CHECK_ARG(n > 0 && n <= INT32_MAX && k > 0 && k <= kMaxK, "%s: n %lld or k %lld out of range", who,
                 static_cast<long long>(n), static_cast<long long>(k));
@@ -1369,41 +911,28 @@ int mtn_w4_matvec(const void* x, int32_t x_dtype, int64_t x_stride, const float*
   mtn::W4Params p{x, x_dtype, x_stride, x_scales, n_rows, static_cast<const uint4*>(packed),
                   static_cast<const uint32_t*>(scales), n, k, group, out, out_dtype, out_stride};
   const int parts = x_dtype == MTN_DTYPE_F32 ? 3 : 1;
+  mtn::MvPlan plan = mtn::mv_plan(n_rows, n, k, group, parts);
   const int elem = x_dtype == MTN_DTYPE_F32 ? 4 : x_dtype == MTN_DTYPE_BF16 ? 2 : 1;
   const int64_t vec = elem == 1 ? 8 : 16;  // bytes of one vector load
-  const int x_vec = reinterpret_cast<uintptr_t>(x) % vec == 0 && (n_rows == 1 || x_stride * elem % vec == 0);
-  auto launch = [&](auto kern, const auto& plan, int threads, size_t smem, int smem_max) {
-    MTN_CUDA_TRY(mtn::allow_smem(reinterpret_cast<const void*>(kern), smem_max), "mtn_w4_matvec");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(plan.clusters * plan.cluster),
-                       static_cast<unsigned>((n_rows + plan.tile - 1) / plan.tile));
-    cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(plan.cluster);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    MTN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, plan), "mtn_w4_matvec");
-    return mtn::check_launch("mtn_w4_matvec");
-  };
-  mtn::TcPlan tc{};
-  if (mtn::tc_plan(n_rows, n, k, x_vec != 0, tc)) {
-    tc.err = mtn::device_error_ptr();
-    int smem = 0;
-    const mtn::TcKernel kern = x_dtype == MTN_DTYPE_F32    ? mtn::tc_kernel<mtn::kXF32>(group, smem)
-                               : x_dtype == MTN_DTYPE_BF16 ? mtn::tc_kernel<mtn::kXBf16>(group, smem)
-                                                           : mtn::tc_kernel<mtn::kXE4m3>(group, smem);
-    return launch(kern, tc, mtn::kTcThreads, static_cast<size_t>(smem), smem);
-  }
-  mtn::MvPlan plan = mtn::mv_plan(n_rows, n, k, group, parts);
-  plan.x_vec = x_vec;
+  plan.x_vec = reinterpret_cast<uintptr_t>(x) % vec == 0 && (n_rows == 1 || x_stride * elem % vec == 0);
   const mtn::MvKernel kern = mtn::mv_kernel(parts, plan.tile > 8 ? 2 : 1, plan.units, group);
-  return launch(kern, plan, mtn::kMvThreads, plan.smem, mtn::kSmemMax);
+  MTN_CUDA_TRY(mtn::allow_smem(reinterpret_cast<const void*>(kern), mtn::kSmemMax), "mtn_w4_matvec");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(plan.clusters * plan.cluster),
+                     static_cast<unsigned>((n_rows + plan.tile - 1) / plan.tile));
+  cfg.blockDim = dim3(mtn::kMvThreads);
+  cfg.dynamicSmemBytes = plan.smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(plan.cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  MTN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, plan), "w4_matvec_kernel");
+  return mtn::check_launch("w4_matvec_kernel");
 }
 
 }  // extern "C"

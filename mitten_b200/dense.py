@@ -184,7 +184,7 @@ def w4_matvec(x: torch.Tensor, weight: W4Weight, *, x_scales: torch.Tensor | Non
 
     x: bf16, f32, or float8_e4m3fn with `x_scales`, one f32 per row (add_rms_norm's e4m3 output).  `out_dtype`
     defaults to x's type, or bf16 for e4m3.  Meant for the few rows of a decode step: the weights are read once
-    per 16 or 32 rows; for a prompt's many rows dequantise and use a matrix product."""
+    per 16 rows; for a prompt's many rows dequantise and use a matrix product."""
     dev = _device_of(x, "x")
     if stream is not None or dev != _current_device():
         with _on(stream, dev):

@@ -96,8 +96,7 @@ def test_general_values(cuda_device, n, k, group, xd, od):
         assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() / tol).max()
 
 
-# More than 16 rows of whole steps of k and 2^22 weights or more go to the tcgen05 products: slices of k over 1 to 8
-# CTAs, tiles that are partly there, a second pass of rows, groups of every size, each of the row types.
+# More than one pass of rows: slices of k over 1 to 8 CTAs, groups of every size, each of the row types.
 @pytest.mark.parametrize("n,k", [(32768, 128), (3584, 1280), (2056, 2048), (18950, 256), (128, 32768), (37888, 384),
                                  (64, 65536), (70, 65536), (4099, 1024)])
 @pytest.mark.parametrize("group,xd", [(32, BF), (64, E4), (128, F32), (128, BF), (32, F32), (64, BF), (32, E4)])
