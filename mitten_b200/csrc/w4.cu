@@ -851,6 +851,7 @@ int mtn_w4_quantize(const void* weight, int32_t dtype, int64_t stride, int64_t n
   MTN_CHECK_ARG(dtype == MTN_DTYPE_BF16 || dtype == MTN_DTYPE_F32, "mtn_w4_quantize: bad dtype");
   MTN_CHECK_ARG(stride >= k, "mtn_w4_quantize: row stride shorter than a row");
   MTN_CHECK_ARG(mtn::aligned16(packed) && mtn::aligned16(scales), "mtn_w4_quantize: packed and scales must be 16-byte aligned");
+  MTN_CHECK_ARG(mtn::elem_aligned(weight, dtype), "mtn_w4_quantize: weight is not aligned to its elements");
   const int64_t blocks = mtn::row_units(n) * (mtn::pad_k(k) / mtn::kKPad);
   mtn::w4_pack_kernel<<<static_cast<unsigned>(blocks), 128, 0, static_cast<cudaStream_t>(stream)>>>(
       weight, dtype, stride, nullptr, 0, nullptr, 0, n, k, group, static_cast<uint4*>(packed),
@@ -865,6 +866,7 @@ int mtn_w4_pack(const int8_t* codes, int64_t code_stride, const void* code_scale
   MTN_CHECK_ARG(codes && code_scales && packed && scales, "mtn_w4_pack: null pointer");
   MTN_CHECK_ARG(code_stride >= k && scale_stride >= (k + group - 1) / group, "mtn_w4_pack: row stride shorter than a row");
   MTN_CHECK_ARG(mtn::aligned16(packed) && mtn::aligned16(scales), "mtn_w4_pack: packed and scales must be 16-byte aligned");
+  MTN_CHECK_ARG(mtn::elem_aligned(code_scales, MTN_DTYPE_BF16), "mtn_w4_pack: code_scales is not aligned to its elements");
   const int64_t blocks = mtn::row_units(n) * (mtn::pad_k(k) / mtn::kKPad);
   mtn::w4_pack_kernel<<<static_cast<unsigned>(blocks), 128, 0, static_cast<cudaStream_t>(stream)>>>(
       nullptr, MTN_DTYPE_F32, 0, codes, code_stride, static_cast<const __nv_bfloat16*>(code_scales), scale_stride, n, k,
@@ -880,6 +882,7 @@ int mtn_w4_dequantize(const void* packed, const void* scales, int64_t n, int64_t
   MTN_CHECK_ARG(dtype == MTN_DTYPE_BF16 || dtype == MTN_DTYPE_F32, "mtn_w4_dequantize: bad dtype");
   MTN_CHECK_ARG(stride >= k, "mtn_w4_dequantize: row stride shorter than a row");
   MTN_CHECK_ARG(mtn::aligned16(packed) && mtn::aligned16(scales), "mtn_w4_dequantize: packed and scales must be 16-byte aligned");
+  MTN_CHECK_ARG(mtn::elem_aligned(out, dtype), "mtn_w4_dequantize: out is not aligned to its elements");
   const int64_t ksteps = mtn::pad_k(k) / mtn::kKPad;
   const int64_t blocks = mtn::row_units(n) * ((ksteps + mtn::kDequantSteps - 1) / mtn::kDequantSteps);
   const int elem = dtype == MTN_DTYPE_BF16 ? 2 : 4;

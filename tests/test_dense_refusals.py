@@ -107,3 +107,15 @@ def test_w4_sizes():
 def test_w4_layout_calls_refuse(call, msg):
     assert call(_lib.lib()) == _lib.MTN_EINVAL
     assert msg in _lib.lib().mtn_last_error()
+
+
+@pytest.mark.parametrize("call", [
+    lambda lib: lib.mtn_w4_quantize(C.c_void_p(0x300002), _lib.MTN_DTYPE_F32, 64, 4, 64, 64, FAKE[0], FAKE[1], None),
+    lambda lib: lib.mtn_w4_quantize(C.c_void_p(0x300001), _lib.MTN_DTYPE_BF16, 64, 4, 64, 64, FAKE[0], FAKE[1], None),
+    lambda lib: lib.mtn_w4_pack(FAKE[2], 64, C.c_void_p(0x400001), 1, 4, 64, 64, FAKE[0], FAKE[1], None),
+    lambda lib: lib.mtn_w4_dequantize(FAKE[0], FAKE[1], 4, 64, 64, C.c_void_p(0x300002), _lib.MTN_DTYPE_F32, 64, None),
+    lambda lib: lib.mtn_w4_dequantize(FAKE[0], FAKE[1], 4, 64, 64, C.c_void_p(0x300001), _lib.MTN_DTYPE_BF16, 64, None),
+])
+def test_w4_layout_calls_refuse_pointers_between_elements(call):
+    assert call(_lib.lib()) == _lib.MTN_EINVAL
+    assert b"not aligned" in _lib.lib().mtn_last_error()
