@@ -522,6 +522,13 @@ int mtn_process_logits(const void* logits, int32_t dtype, int64_t row_stride, in
   MTN_CHECK_ARG(r.mask == nullptr || r.mask_rows != nullptr || r.n_masks >= n_rows,
                 "mtn_process_logits: fewer mask rows than rows, and no mask_rows");
   MTN_CHECK_ARG(r.mask != nullptr || r.mask_rows == nullptr, "mtn_process_logits: mask_rows without a mask");
+  for (const void* q : {static_cast<const void*>(r.hist_indptr), static_cast<const void*>(r.hist_tokens),
+                        static_cast<const void*>(r.prompt_lens), static_cast<const void*>(r.repetition),
+                        static_cast<const void*>(r.presence), static_cast<const void*>(r.frequency),
+                        static_cast<const void*>(r.bias_indptr), static_cast<const void*>(r.bias_tokens),
+                        static_cast<const void*>(r.bias_values), static_cast<const void*>(r.mask),
+                        static_cast<const void*>(r.mask_rows), static_cast<const void*>(tokens)})
+    MTN_CHECK_ARG(reinterpret_cast<uintptr_t>(q) % 4 == 0, "mtn_process_logits: a rule's array or tokens is not aligned to its elements");
   const size_t need = mtn_process_logits_workspace_bytes(n_rows);
   MTN_CHECK_ARG(tokens == nullptr || (workspace != nullptr && workspace_bytes >= need &&
                                       (reinterpret_cast<uintptr_t>(workspace) & 7) == 0),

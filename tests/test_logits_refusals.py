@@ -45,3 +45,25 @@ def test_refuses(kw, msg):
 def test_nothing_to_do():
     assert _call(n=0) == _lib.MTN_OK
     assert _lib.lib().mtn_process_logits_workspace_bytes(5) == 80
+
+
+_HIST = dict(hist_indptr=P[2], hist_tokens=P[3], n_hist=10)
+_BIAS = dict(bias_indptr=P[2], bias_tokens=P[3], bias_values=P[4], n_bias=10)
+_MASK = dict(mask=P[2], mask_stride=4, n_masks=2, mask_rows=P[3])
+
+
+@pytest.mark.parametrize("rules,field", [
+    (_HIST, "hist_indptr"), (_HIST, "hist_tokens"), (dict(_HIST, prompt_lens=P[6]), "prompt_lens"),
+    (dict(_HIST, repetition=P[6]), "repetition"), (dict(_HIST, presence=P[6]), "presence"),
+    (dict(_HIST, frequency=P[6]), "frequency"), (_BIAS, "bias_indptr"), (_BIAS, "bias_tokens"),
+    (_BIAS, "bias_values"), (_MASK, "mask"), (_MASK, "mask_rows"),
+])
+@pytest.mark.parametrize("off", [1, 2])
+def test_refuses_rules_between_elements(rules, field, off):
+    assert _call(rules=dict(rules, **{field: rules[field] + off})) == _lib.MTN_EINVAL
+    assert b"not aligned" in _lib.lib().mtn_last_error()
+
+
+def test_refuses_tokens_between_elements():
+    assert _call(tokens=P[3] + 2, ws=P[4], ws_bytes=64) == _lib.MTN_EINVAL
+    assert b"not aligned" in _lib.lib().mtn_last_error()
