@@ -207,6 +207,7 @@ MTN_API int mtn_qkv_prologue(const mtn_kv_layout* pool, int32_t layer, const voi
  * residual sums of model.rs:348-365), for rows of `hidden` elements (up to
  * 32768), row strides in elements:
  *   sum = x + residual       rounded to res_dtype; sum may be residual itself
+ *                            (with equal strides)
  *   y   = sum / sqrt(mean(sum^2) + eps) * w1      (the sum as it is stored)
  * residual / sum: both NULL for a plain norm of x.  w1: (1 + w) per element,
  * or NULL for ones.  out: bf16 or f32 (scales NULL), or e4m3 with one f32

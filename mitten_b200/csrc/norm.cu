@@ -325,6 +325,8 @@ int mtn_add_rms_norm(const void* x, int32_t x_dtype, int64_t x_stride, const voi
   MTN_CHECK_ARG((out_dtype == MTN_DTYPE_E4M3) == (scales != nullptr),
                 "mtn_add_rms_norm: scales go with an e4m3 output, and only with one");
   MTN_CHECK_ARG(out != x && out != residual && out != sum && sum != x, "mtn_add_rms_norm: outputs overlap the inputs");
+  MTN_CHECK_ARG(residual == nullptr || sum != residual || sum_stride == res_stride || n_rows == 1,
+                "mtn_add_rms_norm: a sum in the residual's place needs equal strides");
   MTN_CHECK_ARG(mtn::elem_aligned(x, x_dtype) && mtn::elem_aligned(out, out_dtype) &&
                     mtn::elem_aligned(residual, res_dtype) && mtn::elem_aligned(sum, res_dtype) &&
                     mtn::elem_aligned(w1, MTN_DTYPE_F32) && mtn::elem_aligned(scales, MTN_DTYPE_F32),

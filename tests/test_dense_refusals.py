@@ -119,3 +119,10 @@ def test_w4_layout_calls_refuse(call, msg):
 def test_w4_layout_calls_refuse_pointers_between_elements(call):
     assert call(_lib.lib()) == _lib.MTN_EINVAL
     assert b"not aligned" in _lib.lib().mtn_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(sum_stride=128), dict(res_stride=128)])
+def test_norm_in_place_needs_equal_strides(kw):
+    # row 1 of the sum would be row 2 of the residual, which another CTA may not have read yet
+    assert _norm(sum_=FAKE[1], n=3, **kw) == _lib.MTN_EINVAL
+    assert b"equal strides" in _lib.lib().mtn_last_error()
