@@ -468,9 +468,13 @@ class Engine:
         ids = np.asarray(prompt, dtype=np.int64)
         if ids.ndim != 1 or ids.size and (ids.min() < 0 or ids.max() >= vocab):
             raise ValueError("prompt must be a list of token ids of the vocabulary")
-        if not rules.repetition > 0 or not np.isfinite([rules.repetition, rules.presence, rules.frequency]).all():
-            raise ValueError("repetition must be positive, and the penalties finite")
-        if any(not 0 <= t < vocab for t in rules.bias) or not all(v < np.inf for v in rules.bias.values()):
+        with np.errstate(over="ignore", divide="ignore"):  # the values as the kernel has them
+            rep, pres, freq = np.array([rules.repetition, rules.presence, rules.frequency], np.float32)
+            bias = np.array(list(rules.bias.values()), np.float32)
+            usable = rep > 0 and np.isfinite([rep, np.float32(1) / rep, pres, freq]).all()
+        if not usable:
+            raise ValueError("repetition must be positive with a finite reciprocal, and the penalties finite, in f32")
+        if any(not 0 <= t < vocab for t in rules.bias) or not (bias < np.inf).all():
             raise ValueError("bias: token ids of the vocabulary with values that are numbers below infinity")
         self._rules[int(req_id)] = (ids.astype(np.int32), rules)
 
