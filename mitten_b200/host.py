@@ -10,6 +10,7 @@ tests read the same against this module:
 from __future__ import annotations
 
 import ctypes as C
+from collections.abc import Callable
 from dataclasses import dataclass
 
 import numpy as np
@@ -191,6 +192,7 @@ class Scheduler:
         self._h = h
         self._destroy = L.lib().mtn_sched_destroy
         self.page_size = page_size
+        self.on_export: list[Callable[[int], object]] = []  # called with the id of each request that leaves by export
 
     def __del__(self):
         # the destroy function is bound at construction: module globals may
@@ -262,6 +264,8 @@ class Scheduler:
         pages, outs = (C.c_uint32 * npg)(), (C.c_uint32 * nout)()
         n_p, n_o, dl = C.c_int64(npg), C.c_int64(nout), C.c_int64()
         L.check(L.lib().mtn_sched_export(self._h, req_id, pages, C.byref(n_p), C.byref(dl), outs, C.byref(n_o)))
+        for f in self.on_export:
+            f(int(req_id))
         return {"pages": list(pages[:n_p.value]), "device_len": dl.value, "outputs": list(outs[:n_o.value])}
 
     def import_request(self, req_id: int, input_ids, outputs, device_len: int, temperature: float = 0.0,

@@ -33,6 +33,7 @@ matrix and multiply.  `act_e4m3` hands the norms' rows on in 8 bits.
 """
 from __future__ import annotations
 
+import weakref
 from collections.abc import Callable
 from dataclasses import dataclass, field
 
@@ -461,9 +462,13 @@ class Engine:
         self._sample_ws = None
         self._rules: dict[int, tuple[np.ndarray, TokenRules]] = {}
         self._rules_ws = None
+        me = weakref.ref(self)
+        sched.on_export.append(lambda req_id: me() is not None and me()._rules.pop(req_id, None))
 
     def set_rules(self, req_id: int, prompt, rules: TokenRules) -> None:
-        """Penalties, biases and masks for a queued request; `prompt` is what it was queued with."""
+        """Penalties, biases and masks for a queued request; `prompt` is what it was queued with.
+
+        They end with the request, also when it is exported: after an import they have to be given again."""
         vocab = self.model.s.vocab
         ids = np.asarray(prompt, dtype=np.int64)
         if ids.ndim != 1 or ids.size and (ids.min() < 0 or ids.max() >= vocab):
@@ -542,15 +547,20 @@ class Engine:
         lost = logits.gather(1, tokens.long()[:, None])[:, 0].isneginf() | ~torch.isfinite(top)
         return torch.where(ruled & lost, picked, tokens)
 
-    def _drop_rules(self, b) -> None:
-        """Forget the rules of requests that have ended."""
-        for r in b.req_ids:
-            if int(r) in self._rules and self.sched.request_info(int(r))["state"] in (L.MTN_REQ_DONE, L.MTN_REQ_ABORTED):
-                del self._rules[int(r)]
+    def _drop_rules(self) -> None:
+        """Forget the rules of requests that have ended, in a batch or as one was made."""
+        for r in list(self._rules):
+            try:
+                ended = self.sched.request_info(r)["state"] in (L.MTN_REQ_DONE, L.MTN_REQ_ABORTED)
+            except L.MittenError:  # not queued yet
+                continue
+            if ended:
+                del self._rules[r]
 
     def step(self) -> bool:
         b = self.sched.schedule()
         if b is None:
+            self._drop_rules()
             return False
         try:
             logits = self.model.decode_step(b) if self.cuda_graphs else self.model.forward(b)
@@ -574,11 +584,10 @@ class Engine:
                                     f"device error {code} (detail {detail}) in the step's kernels")
         except (L.MittenError, RuntimeError):
             self.sched.abort_batch()
-            self._drop_rules(b)
+            self._drop_rules()
             raise
         self.sched.process_tokens(tokens)
-        if self._rules:
-            self._drop_rules(b)
+        self._drop_rules()
         self.iterations += 1
         return True
 

@@ -1,19 +1,41 @@
-"""The engine's token rules on the host: what set_rules refuses (CPU: a stand-in for the model, nothing launched)."""
+"""The engine's token rules on the host: what set_rules refuses, and whose rules a step applies (CPU: stand-ins for
+the model and the kernels, nothing launched)."""
 from __future__ import annotations
 
 from types import SimpleNamespace
 
 import numpy as np
 import pytest
+import torch
 
-from mitten_b200 import host, model as M
+from mitten_b200 import _lib, host, model as M
 
 VOCAB = 64
 
 
-def _engine(**kw):
-    sched = host.Scheduler(64, 16, eos_token_ids=(VOCAB,), **kw)
-    return M.Engine(SimpleNamespace(s=SimpleNamespace(vocab=VOCAB)), sched, cuda_graphs=False), sched
+def _engine(pages=64, page_size=16, **kw):
+    sched = host.Scheduler(pages, page_size, eos_token_ids=(VOCAB,), **kw)
+    model = SimpleNamespace(s=SimpleNamespace(vocab=VOCAB), dev=SimpleNamespace(index=0),
+                            forward=lambda b: torch.zeros(b.n_reqs, VOCAB))
+    return M.Engine(model, sched, cuda_graphs=False), sched
+
+
+@pytest.fixture
+def applied(monkeypatch):
+    """The rules of every step that applied some, as its keyword arguments; every row's token is 1."""
+    calls = []
+
+    def rules(**kw):
+        calls.append({k: v.tolist() for k, v in kw.items()})
+
+    def pick(logits, *args, **kw):
+        return torch.ones(len(logits), dtype=torch.int32)
+
+    monkeypatch.setattr(M.paged, "LogitsRules", rules)
+    monkeypatch.setattr(M.paged, "process_logits", lambda logits, *a, **kw: (logits, pick(logits)))
+    monkeypatch.setattr(M.paged, "argmax_rows", pick)
+    monkeypatch.setattr(M.paged, "device_error", lambda dev: (0, 0))
+    return calls
 
 
 @pytest.mark.parametrize("rules", [
@@ -38,3 +60,45 @@ def test_values_within_f32_are_taken(rules):
     eng, _ = _engine()
     eng.set_rules(0, np.arange(3), rules)
     assert 0 in eng._rules
+
+
+def test_rules_end_with_an_exported_request(applied):
+    eng, sched = _engine()
+    sched.add_request(7, np.arange(5, dtype=np.uint32), max_new_tokens=8)
+    eng.set_rules(7, np.arange(5), M.TokenRules(presence=1.0))
+    eng.step()
+    assert len(applied) == 1
+    h = sched.export_request(7)
+    assert not eng._rules
+    # another request under the same id, as a handoff from elsewhere brings it
+    sched.import_request(7, [9, 9, 9], h["outputs"], 3, 0.0, 8)
+    eng.step()
+    assert len(applied) == 1
+    # its own rules, given after the import, do apply
+    eng.set_rules(7, [9, 9, 9], M.TokenRules(presence=1.0))
+    eng.step()
+    assert len(applied) == 2 and applied[1]["hist_tokens"] == [9, 9, 9] + h["outputs"] + [1]
+
+
+def test_rules_end_with_a_request_that_no_batch_holds(applied):
+    """A request that finds no page for its next token is aborted as the batch is made, and is not part of it."""
+    eng, sched = _engine(pages=4, page_size=4)
+    for rid, n in ((0, 4), (1, 12)):
+        sched.add_request(rid, np.arange(n, dtype=np.uint32) + 20 * rid, max_new_tokens=8)
+        eng.set_rules(rid, np.arange(n) + 20 * rid, M.TokenRules(presence=1.0))
+    while sched.num_active():
+        eng.step()
+        for rid in (0, 1):
+            live = sched.request_info(rid)["state"] not in (_lib.MTN_REQ_DONE, _lib.MTN_REQ_ABORTED)
+            assert (rid in eng._rules) == live
+    assert _lib.MTN_REQ_ABORTED in [sched.request_info(r)["state"] for r in (0, 1)]
+
+
+def test_rules_given_before_their_request_is_queued_are_kept(applied):
+    eng, sched = _engine()
+    eng.set_rules(3, [1, 2], M.TokenRules(presence=1.0))
+    sched.add_request(0, np.arange(2, dtype=np.uint32), max_new_tokens=1)
+    eng.step()
+    sched.add_request(3, np.array([1, 2], np.uint32), max_new_tokens=2)
+    eng.run()
+    assert len(applied) == 2 and not eng._rules
