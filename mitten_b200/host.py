@@ -192,6 +192,7 @@ class Scheduler:
         self._h = h
         self._destroy = L.lib().mtn_sched_destroy
         self.page_size = page_size
+        self._prompt_lens: dict[int, int] = {}
         self.on_export: list[Callable[[int], object]] = []  # called with the id of each request that leaves by export
 
     def __del__(self):
@@ -204,6 +205,7 @@ class Scheduler:
     def add_request(self, req_id: int, input_ids, temperature: float = 0.0, max_new_tokens: int = 512) -> None:
         a, p = _u32(input_ids)
         L.check(L.lib().mtn_sched_add_request(self._h, req_id, p, len(a), temperature, max_new_tokens))
+        self._prompt_lens[int(req_id)] = len(a)
 
     def schedule(self) -> Batch | None:
         v = L.BatchView()
@@ -238,6 +240,10 @@ class Scheduler:
         return {"state": st.value, "device_len": dl.value, "cached_len": cl.value, "n_pages": npg.value,
                 "n_output": nout.value}
 
+    def prompt_len(self, req_id: int) -> int:
+        """Tokens of the prompt that a request was queued with (a fork's: its parent's and the suffix)."""
+        return self._prompt_lens[int(req_id)]
+
     def request_pages(self, req_id: int) -> list[int]:
         n = self.request_info(req_id)["n_pages"]
         buf = (C.c_uint32 * max(n, 1))()
@@ -256,6 +262,7 @@ class Scheduler:
         """Queue child_id = parent's prompt + suffix, sharing the parent's prompt pages (refcount mode)."""
         a, p = _u32(suffix)
         L.check(L.lib().mtn_sched_fork(self._h, parent_id, child_id, p, len(a), temperature, max_new_tokens))
+        self._prompt_lens[int(child_id)] = self._prompt_lens[int(parent_id)] + len(a)
 
     def export_request(self, req_id: int) -> dict:
         """Hand a decoding request over (KvHandoff): its pages, device_len and generated tokens."""
@@ -278,6 +285,7 @@ class Scheduler:
         n = C.c_int64(max(cap, 1))
         L.check(L.lib().mtn_sched_import(self._h, req_id, ap, len(a), op, len(o), device_len, temperature,
                                          max_new_tokens, pages, C.byref(n)))
+        self._prompt_lens[int(req_id)] = len(a)
         return list(pages[:n.value])
 
     def page_refcount(self, page: int) -> int:

@@ -439,7 +439,7 @@ class TokenRules:
     presence: float = 0.0     # subtracted once from every generated token
     frequency: float = 0.0    # subtracted per occurrence among the generated tokens
     bias: dict[int, float] = field(default_factory=dict)
-    # generated tokens so far -> [vocab] truth values of the tokens allowed next, or None for all
+    # generated tokens so far -> [vocab] truth values of the tokens allowed next, or None for all; asked once a token
     allowed: Callable[[list[int]], np.ndarray | None] | None = None
 
 
@@ -484,9 +484,11 @@ class Engine:
         self._rules[int(req_id)] = (ids.astype(np.int32), rules)
 
     def _apply_rules(self, b, logits: torch.Tensor) -> torch.Tensor:
-        """The batch's rules on its logits, in place; the greedy tokens.  Rows without rules pass as they are."""
+        """The batch's rules on its logits, in place; the greedy tokens.  Rows without rules pass as they are, and so
+        do those of unfinished prompt chunks, whose token the scheduler throws away."""
         n, vocab = logits.shape
-        mine = [self._rules.get(int(r)) for r in b.req_ids]
+        mine = [None if i < b.n_prefill and b.seq_lens[i] < self.sched.prompt_len(r) else self._rules.get(int(r))
+                for i, r in enumerate(b.req_ids)]
         out = [self.sched.request_output(int(r)) if m else [] for r, m in zip(b.req_ids, mine)]
         none = (np.zeros(0, np.int32), TokenRules())
         hist = [np.concatenate([m[0], np.asarray(o, np.int32)]) if m else none[0] for m, o in zip(mine, out)]

@@ -102,3 +102,33 @@ def test_rules_given_before_their_request_is_queued_are_kept(applied):
     sched.add_request(3, np.array([1, 2], np.uint32), max_new_tokens=2)
     eng.run()
     assert len(applied) == 2 and not eng._rules
+
+
+def test_allowed_is_asked_once_for_every_token(applied):
+    """A prompt in chunks of 16: the rows of its unfinished chunks give no token."""
+    eng, sched = _engine(max_prefill_tokens_per_iter=16)
+    asked = {0: [], 1: [], 2: []}
+
+    def allowed(rid):
+        return lambda out: asked[rid].append(list(out))
+
+    def queue(rid, prompt):
+        eng.set_rules(rid, prompt, M.TokenRules(allowed=allowed(rid), presence=1.0))
+
+    sched.add_request(0, np.arange(40, dtype=np.uint32), max_new_tokens=6)
+    queue(0, np.arange(40))
+    eng.step()
+    eng.step()
+    assert asked[0] == [] and all(a["hist_tokens"] == [] for a in applied)
+    eng.step()
+    assert asked[0] == [[]] and applied[-1]["hist_tokens"] == list(range(40))
+    # a fork's prompt is its parent's and the suffix; its chunks run beside the parent's tokens
+    sched.fork(0, 1, np.arange(20, dtype=np.uint32), max_new_tokens=3)
+    queue(1, np.concatenate([np.arange(40), np.arange(20)]))
+    eng.run()
+    assert asked[0] == [[1] * i for i in range(6)] and asked[1] == [[1] * i for i in range(3)]
+    # an imported request has its prompt behind it
+    sched.import_request(2, np.arange(5), [1, 1], 6, 0.0, 4)
+    queue(2, np.arange(5))
+    eng.run()
+    assert asked[2] == [[1, 1], [1, 1, 1]]
