@@ -212,7 +212,7 @@ MTN_API int mtn_qkv_prologue(const mtn_kv_layout* pool, int32_t layer, const voi
  * residual / sum: both NULL for a plain norm of x.  w1: (1 + w) per element,
  * or NULL for ones.  out: bf16 or f32 (scales NULL), or e4m3 with one f32
  * scale per row, scale = max(max|y| / 448, 2^-100), out = e4m3(y / scale).
- * Means and y are f32; a row that holds a NaN or an infinity comes out as
+ * Means, y and y / scale are f32; a row that holds a NaN or an infinity comes out as
  * the formula says, NaN scale included.  Besides sum == residual no output
  * may overlap an input. */
 MTN_API int mtn_add_rms_norm(const void* x, int32_t x_dtype, int64_t x_stride, const void* residual,

@@ -169,3 +169,34 @@ def test_wrapper_refuses(cuda_device):
     with pytest.raises(ValueError):  # rows that share memory
         dense.add_rms_norm(torch.zeros(64, device="cuda").expand(4, 64))
     assert paged.device_error(0) == (0, 0)
+
+
+@pytest.mark.parametrize("hidden", [256, 259, 2048, 2055])
+@pytest.mark.parametrize("xd", [BF, F32])
+def test_e4m3_codes_are_those_of_the_quotient(cuda_device, hidden, xd):
+    """Rows of signs with eps 0 have y = w1, exactly, and with a scale s of 16 bits w1 = 448 s and w1 = t s are exact
+    for every t halfway between two codes: y / s is t without rounding, and the code is the even neighbour's."""
+    codes = torch.arange(0x7f, dtype=torch.uint8).view(E4).float()  # every finite value from 0 on
+    half = (codes[:-1] + codes[1:]) / 2
+    want = half.to(E4).float()
+    g = torch.Generator().manual_seed(hidden)
+    sign = torch.randint(0, 2, (3, hidden), generator=g).float() * 2 - 1
+    at = torch.arange(hidden - 1) % len(half)
+    for s in torch.randint(1 << 15, 1 << 16, (40,), generator=g).tolist():
+        s *= 2.0 ** -20
+        w1 = torch.cat([torch.tensor([448.0]), half[at]]) * s
+        out, scales = dense.add_rms_norm(sign.to(xd).cuda(), w1.cuda(), 0.0, out_dtype=E4)
+        assert (scales == s).all()
+        assert torch.equal(out.float().cpu(), sign * torch.cat([torch.tensor([448.0]), want[at]]))
+
+
+@pytest.mark.parametrize("hidden", [256, 259, 2048])
+def test_e4m3_rows_of_infinite_values(cuda_device, hidden):
+    x = torch.ones(2, hidden, device="cuda")
+    x[1] = -1.0
+    w1 = torch.rand(hidden, device="cuda") + 0.5
+    w1[3] = float("inf")
+    out, scales = dense.add_rms_norm(x, w1, 0.0, out_dtype=E4)
+    assert (scales == float("inf")).all()  # the quotients: 0, and NaN for infinity over infinity
+    o = out.float()
+    assert o[:, 3].isnan().all() and (o[:, :3] == 0).all() and (o[:, 4:] == 0).all()
