@@ -287,3 +287,28 @@ def test_sampling_with_rules_keeps_to_them(cuda_device, monkeypatch):
     with pytest.raises(ValueError):
         M.Engine(model, host.Scheduler(64, 16, eos_token_ids=(cfg.vocab,))).set_rules(
             0, [1], M.TokenRules(bias={1: float("inf")}))
+
+
+@pytest.mark.parametrize("act_e4m3", [False, True])
+def test_head_of_many_rows_keeps_f32_logits(cuda_device, act_e4m3):
+    """A bf16 model's head above the row limit of the matrix-vector product.  Scales that are powers of two leave
+    the dequantised weights exact in bf16, as bf16 and e4m3 rows are: what is left to round are the f32 sums, each
+    of their k additions by at most 2 u of the magnitudes' sum (a tensor core may cut), and one product."""
+    cfg = R.QwenShape(hidden=256, layers=1, hq=14, hkv=2, head_dim=64, inter=512, vocab=5003)
+    model = M.QwenPagedModel(shape_of(cfg), R.random_weights(cfg, seed=3), 64, 16, dtype=torch.bfloat16, w4_group=64,
+                             act_e4m3=act_e4m3)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    codes = torch.randint(-8, 8, (cfg.vocab, cfg.hidden), generator=g, device="cuda", dtype=torch.int8)
+    scales = 2.0 ** torch.randint(-8, -3, (cfg.vocab, 4), generator=g, device="cuda").float()
+    model.q4["head"] = dense.W4Weight.from_codes(codes, scales.to(torch.bfloat16), 64)
+    for rows in (M.W4_MATVEC_ROWS[torch.bfloat16], M.W4_MATVEC_ROWS[torch.bfloat16] + 1, 200):
+        x = torch.randn(rows, cfg.hidden, generator=g, device="cuda")
+        xs = x.abs().amax(1) / 448.0 if act_e4m3 else None
+        x = (x / xs[:, None]).to(torch.float8_e4m3fn) if act_e4m3 else x.to(torch.bfloat16)
+        got = model._linear4("head", x, xs, out_dtype=torch.float32)
+        assert got.dtype == torch.float32 and got.is_contiguous()
+        xv = x.double() if xs is None else x.double() * xs.double()[:, None]
+        val = codes.double() * scales.double().repeat_interleave(64, 1)
+        want, mag = xv @ val.T, xv.abs() @ val.abs().T
+        u = 2.0 ** -24
+        assert ((got.double() - want).abs() <= 2 * cfg.hidden * u * mag + 2 * u * want.abs()).all(), rows
