@@ -312,3 +312,66 @@ def test_head_of_many_rows_keeps_f32_logits(cuda_device, act_e4m3):
         want, mag = xv @ val.T, xv.abs() @ val.abs().T
         u = 2.0 ** -24
         assert ((got.double() - want).abs() <= 2 * cfg.hidden * u * mag + 2 * u * want.abs()).all(), rows
+
+
+def test_w4_model_without_the_fused_prologue(cuda_device):
+    """q, k and v as strided parts of one product, through torch's norms, RoPE and a separate append."""
+    cfg = R.QwenShape(hidden=256, layers=3, hq=14, hkv=2, head_dim=64, inter=512, vocab=4096)
+    w = _quantised(R.random_weights(cfg, seed=64), 64)
+    rng = np.random.default_rng(1)
+    prompts = [rng.integers(0, cfg.vocab, n).astype(np.int64) for n in (40, 17, 130, 5)]
+    want = R.generate(R.RefModel(cfg, w, kv_round=True), prompts, 8)
+    for graphs in (False, True):
+        eng, sched = _engine(cfg, w, prompts, 8, graphs, w4_group=64, fused_prologue=False)
+        eng.run()
+        assert [sched.request_output(r) for r in range(len(prompts))] == want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act_e4m3", [False, True])
+@pytest.mark.parametrize("lens", [(30, 9, 6), (150, 40, 7)])
+def test_w4_model_in_each_type_and_for_many_rows(cuda_device, monkeypatch, dtype, act_e4m3, lens):
+    """The model against itself with its norms and its 4-bit products replaced by plain torch in f32, rounded to the
+    model's type where the model rounds; 45 rows go through the matrix-vector product, 197 through dequantised
+    matrices.  f32: a code of e4m3 comes out differently for about 2e-5 of the elements and then moves its row by 1 %
+    of its length at most; two such may meet in a row.  bf16: two layers and the head round about 24 times, each by at
+    most 2^-8 of a row's length.  With e4m3 rows a value off by 2^-8 gets another code, 2^-4 off, in one case of 16 at
+    most: a quarter of 2^-4 for each of 5 norms."""
+    cfg = R.QwenShape(hidden=256, layers=2, hq=14, hkv=2, head_dim=64, inter=512, vocab=4096)
+    w = R.random_weights(cfg, seed=5)
+    rng = np.random.default_rng(6)
+    prompts = [rng.integers(0, cfg.vocab, n).astype(np.int64) for n in lens]
+
+    def logits():
+        eng, sched = _engine(cfg, w, prompts, 4, False, w4_group=64, act_e4m3=act_e4m3, dtype=dtype)
+        out = []
+        while sched.num_active():
+            b = sched.schedule()
+            out.append(eng.model.forward(b))
+            sched.process_tokens((np.arange(b.n_reqs) * 7 + len(out)).astype(np.uint32))  # the same tokens for both
+        return out
+
+    def norm(x, w1, eps, residual=None, out_dtype=None):
+        if residual is not None:
+            residual.copy_(residual.float() + x.float())
+            x = residual
+        x = x.float()
+        y = x / torch.sqrt(x.square().mean(1, keepdim=True) + eps) * w1
+        if out_dtype != torch.float8_e4m3fn:
+            return y.to(out_dtype), None
+        scale = (y.abs().amax(1) / 448.0).clamp(min=2.0 ** -100)
+        return (y / scale[:, None]).clamp(-448, 448).to(out_dtype), scale
+
+    def linear(model, name, x, scales=None, out_dtype=None):
+        x = x.float() if scales is None else x.float() * scales[:, None]
+        return (x @ model.q4[name].dequantize().T).to(out_dtype or model.dt)
+
+    got = logits()
+    monkeypatch.setattr(M.dense, "add_rms_norm", norm)
+    monkeypatch.setattr(M.QwenPagedModel, "_linear4", linear)
+    want = logits()
+    tol = 2e-2 if dtype == torch.float32 else 24 * 2.0 ** -8 + (5 * 2.0 ** -6 if act_e4m3 else 0.0)
+    assert len(got) == len(want) > 2
+    for a, b in zip(got, want):
+        assert a.dtype == torch.float32
+        assert ((a - b).norm() <= tol * b.norm()), ((a - b).norm() / b.norm())
