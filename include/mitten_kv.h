@@ -429,7 +429,8 @@ MTN_API int mtn_sample_rows(const float* logits, const float* temperatures, int6
  *     NULL: mask row r).
  * Token ids outside the vocabulary are skipped, a malformed index pointer
  * counts as an empty row and a mask row out of range as none, each recorded
- * as device error 7. */
+ * as device error 7 (an index pointer over a list without entries is not
+ * looked at).  Pointers are aligned to their elements. */
 typedef struct {
   const int32_t* hist_indptr;
   const int32_t* hist_tokens;
@@ -453,9 +454,10 @@ typedef struct {
  *   x = in the history ? (x > 0 ? x / repetition : x * repetition) : x
  *   x = x - frequency * (times generated);  x = x - presence if generated
  *   x = x + bias;  x = allowed ? x : -inf
- * out may be logits (f32, equal strides).  tokens (or NULL): the processed
- * row's first strict maximum, as mtn_argmax_rows gives it (a row whose mask
- * leaves nothing gives 0).  workspace: for tokens only,
+ * out may be logits (f32, equal strides) and must not overlap them otherwise.
+ * tokens (or NULL): the processed row's first strict maximum, as
+ * mtn_argmax_rows gives it (a row whose mask leaves nothing gives 0).
+ * workspace: for tokens only,
  * mtn_process_logits_workspace_bytes(n_rows) bytes, 8-byte aligned, zeroed
  * once before first use and left zeroed by every call, one stream at a time.
  * scratch: for a history or biases only,

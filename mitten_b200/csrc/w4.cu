@@ -18,7 +18,8 @@
 //   word 2: row g + 8, k = 8 t + 0..7       word 3: row g + 8, k = 32 + 8 t + 0..7
 // and element j of a word's eight sits in nibble (j >> 1) + 4 (j & 1), two's
 // complement: shifted right by 4 p and masked with 0x000f000f a word gives
-// the neighbours k = 2p, 2p + 1 in its two halves.  Units follow one another
+// the neighbours k = 2p, 2p + 1 in its two halves (integers made floats by an
+// exponent set beside them: Kim, Henry, Fahim, Awadalla, 2022).  Units follow one another
 // along k, then along the rows.  Scales: [row unit][k / G][8] words, word g
 // holding row g's scale in its low half and row g + 8's in its high half.
 #include <algorithm>
@@ -63,7 +64,9 @@ __device__ __forceinline__ int code_of(uint32_t w, int j) {
 // every row.  From float weights (codes == null) it first quantises: per
 // group s = bf16(max|w| / 7), q = round(w / s) to -8..7, so that the codes
 // are those of the scale as stored; a group of zeros has scale 0, one that
-// holds a NaN or an infinity a NaN scale (its products then are NaN).
+// holds a NaN or an infinity a NaN scale (its products then are NaN).  Runs once
+// a weight and was not made faster: 18944 x 3584 takes 430 us from floats (two
+// barriers a row) and 160 from codes.
 __global__ void __launch_bounds__(128) w4_pack_kernel(const void* w, int dtype, int64_t stride, const int8_t* codes,
                                                       int64_t code_stride, const __nv_bfloat16* in_scales,
                                                       int64_t scale_stride, int64_t n, int64_t k, int group,
@@ -208,8 +211,12 @@ struct W4Params {
 // alone would each take about 48, so the two no longer hide each other
 // entirely.  A matrix of 34 MB (18944 x 3584) takes 10.0 us against 5.3 for
 // its bytes: start (instructions, x, the first weights) 2 us, join and drain
-// 1.5.  16 rows take 80 us for the 152064 rows: mma.sync runs at half of what
-// the two tiles of x rows need, and neither loads nor unpacking matter.
+// 1.5.  16 rows take 78 us for the 152064 rows (16.3 for 18944) and no unit is
+// full: issue slots are 55 % used, ALUs 40 %, the tensor pipe 24 %, DRAM 21 %, and
+// a version without the unpacking, without x loads or without the weights' loads
+// took 66, 66 and 65 us (of 76).  Warps wait for fixed latencies (1.8 of 7.3 warps
+// a cycle) and for math pipes (1.3): 16 warps of 128 registers, with 36 to 68 bytes
+// spilled, hide too little of chains of two dependent products.
 //
 // f32 rows are cut into three bf16 parts of 8 bits each, which hold all 24
 // bits, and multiplied part by part into the same sums.

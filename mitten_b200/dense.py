@@ -183,8 +183,10 @@ def w4_matvec(x: torch.Tensor, weight: W4Weight, *, x_scales: torch.Tensor | Non
     """x [m, k] times the transposed 4-bit weight: [m, n] in bf16 or f32 (mtn_w4_matvec), sums in f32.
 
     x: bf16, f32, or float8_e4m3fn with `x_scales`, one f32 per row (add_rms_norm's e4m3 output).  `out_dtype`
-    defaults to x's type, or bf16 for e4m3.  Meant for the few rows of a decode step: the weights are read once
-    per 16 rows; for a prompt's many rows dequantise and use a matrix product."""
+    defaults to x's type, or bf16 for e4m3.  Meant for the few rows of a decode step: the weights are read at
+    least once per 16 rows, and more often where so many rows do not fit in shared memory (16 f32 rows of 18944);
+    for a prompt's many rows dequantise and use a matrix product.  The order of the sums goes by the number of
+    rows."""
     dev = _device_of(x, "x")
     if stream is not None or dev != _current_device():
         with _on(stream, dev):
