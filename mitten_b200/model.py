@@ -121,6 +121,7 @@ class QwenPagedModel:
         # (1 + w) of the layer norms in f32, and the 4-bit matrices
         self.q4: dict[str, dense.W4Weight] = {}
         self.w1: dict[str, torch.Tensor] = {}
+        self._values: dict[bool, torch.Tensor] = {}
         if w4_group is not None:
             self._quantize(w4_group)
         # RMSNorm scales (1 + w), formed once
@@ -163,13 +164,22 @@ class QwenPagedModel:
         self.q4["head"] = dense.W4Weight.from_float(w["embedding.weight"].contiguous(), group)
 
     # ------------------------------------------------------------ pieces
+    def _dequantized(self, name: str, w: dense.W4Weight) -> torch.Tensor:
+        """A 4-bit matrix in the model's type, until the next one is asked for: one buffer serves the layers and one
+        the head, so that captured graphs do not each hold the largest matrix."""
+        kind = name == "head"
+        if kind not in self._values:
+            most = max(q.n * q.k for k, q in self.q4.items() if (k == "head") == kind)
+            self._values[kind] = torch.empty(most, dtype=self.dt, device=self.dev)
+        return w.dequantize(out=self._values[kind][:w.n * w.k].view(w.n, w.k))
+
     def _linear4(self, name: str, x: torch.Tensor, scales: torch.Tensor | None = None,
                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
         """x @ W.T for a 4-bit matrix; x in the model's type, or e4m3 with a scale per row."""
         w, out_dtype = self.q4[name], out_dtype or self.dt
         if x.shape[0] <= W4_MATVEC_ROWS[self.dt]:
             return dense.w4_matvec(x, w, x_scales=scales, out_dtype=out_dtype)
-        wt = w.dequantize(self.dt).T
+        wt = self._dequantized(name, w).T
         if out_dtype != self.dt:  # a bf16 model's logits: f32 sums as they are, and exact e4m3 rows
             y = torch.mm(x.to(self.dt), wt, out_dtype=out_dtype)
             return y if scales is None else y.mul_(scales[:, None])

@@ -375,3 +375,33 @@ def test_w4_model_in_each_type_and_for_many_rows(cuda_device, monkeypatch, dtype
     for a, b in zip(got, want):
         assert a.dtype == torch.float32
         assert ((a - b).norm() <= tol * b.norm()), ((a - b).norm() / b.norm())
+
+
+def test_graphs_of_many_rows_share_the_dequantised_matrices(cuda_device):
+    """A decode graph of more rows than the matrix-vector product takes dequantises matrices: graphs of other batch
+    sizes must not each keep a copy.  The head is 105 MB in bf16, a graph's own logits are 21 MB."""
+    cfg = R.QwenShape(hidden=512, layers=1, hq=14, hkv=2, head_dim=64, inter=512, vocab=102400)
+    rng = np.random.default_rng(2)
+    head = cfg.vocab * cfg.hidden * 2
+    first, n = M.W4_MATVEC_ROWS[torch.bfloat16] + 1, 6
+    model = M.QwenPagedModel(shape_of(cfg), R.random_weights(cfg, seed=2), 256, 16, dtype=torch.bfloat16, w4_group=64)
+    prompts = [rng.integers(0, cfg.vocab, 5).astype(np.uint32) for _ in range(first + n)]
+
+    def tokens(size):
+        sched = host.Scheduler(256, 16, max_prefill_tokens_per_iter=512, max_decode_batch_size=64, eos_token_ids=(cfg.vocab,))
+        for r in range(size):
+            sched.add_request(r, prompts[r], max_new_tokens=4)
+        M.Engine(model, sched).run()
+        return [sched.request_output(r) for r in range(size)]
+
+    def held():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return torch.cuda.memory_reserved()
+
+    want = tokens(first)
+    before = held()
+    for i in range(1, n + 1):
+        assert tokens(first + i)[:first] == want
+    assert held() - before < n * head
+    assert tokens(first) == want  # the first graph again, replayed from its first decode step on
