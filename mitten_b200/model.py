@@ -573,9 +573,9 @@ class Engine:
         lost = logits.gather(1, tokens.long()[:, None])[:, 0].isneginf() | ~torch.isfinite(top)
         return torch.where(ruled & lost, picked, tokens)
 
-    def _drop_rules(self) -> None:
-        """Forget the rules of requests that have ended, in a batch or as one was made."""
-        for r in list(self._rules):
+    def _drop_rules(self, req_ids) -> None:
+        """Forget the rules of those requests that have ended."""
+        for r in [int(r) for r in req_ids if int(r) in self._rules]:
             try:
                 ended = self.sched.request_info(r)["state"] in (L.MTN_REQ_DONE, L.MTN_REQ_ABORTED)
             except L.MittenError:  # not queued yet
@@ -584,9 +584,11 @@ class Engine:
                 del self._rules[r]
 
     def step(self) -> bool:
+        active = self.sched.num_active()
         b = self.sched.schedule()
+        if self._rules and self.sched.num_active() < active:  # requests without a page for their next token
+            self._drop_rules(list(self._rules))
         if b is None:
-            self._drop_rules()
             return False
         try:
             logits = self.model.decode_step(b) if self.cuda_graphs else self.model.forward(b)
@@ -610,10 +612,10 @@ class Engine:
                                     f"device error {code} (detail {detail}) in the step's kernels")
         except (L.MittenError, RuntimeError):
             self.sched.abort_batch()
-            self._drop_rules()
+            self._drop_rules(b.req_ids)
             raise
         self.sched.process_tokens(tokens)
-        self._drop_rules()
+        self._drop_rules(b.req_ids)
         self.iterations += 1
         return True
 

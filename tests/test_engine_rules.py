@@ -132,3 +132,18 @@ def test_allowed_is_asked_once_for_every_token(applied):
     queue(2, np.arange(5))
     eng.run()
     assert asked[2] == [[1, 1], [1, 1, 1]]
+
+
+def test_a_step_looks_only_at_its_own_requests(applied, monkeypatch):
+    """Rules of queued requests cost a step nothing: their state is not asked for."""
+    eng, sched = _engine(max_prefill_tokens_per_iter=4)
+    for rid in range(50):
+        sched.add_request(rid, np.arange(4, dtype=np.uint32), max_new_tokens=2)
+        eng.set_rules(rid, np.arange(4), M.TokenRules(presence=1.0))
+    asked = []
+    info = sched.request_info
+    monkeypatch.setattr(sched, "request_info", lambda r: asked.append(r) or info(r))
+    eng.step()
+    assert set(asked) == {0}
+    eng.run()
+    assert not eng._rules and all(len(sched.request_output(r)) == 2 for r in range(50))
