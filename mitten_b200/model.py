@@ -39,6 +39,7 @@ is memory.
 """
 from __future__ import annotations
 
+import gc
 import weakref
 from collections.abc import Callable
 from dataclasses import dataclass, field
@@ -403,7 +404,7 @@ class _DecodeGraph:
 
     def __init__(self, model: QwenPagedModel, n: int):
         dev = model.dev
-        self.model, self.n = model, n
+        self.model, self.n = weakref.proxy(model), n  # the model holds its graphs: no cycle for the collector
         self.ids = torch.zeros(n, dtype=torch.int64, device=dev)
         self.pos = torch.zeros(n, dtype=torch.int32, device=dev)
         self.kv_indptr = torch.zeros(n + 1, dtype=torch.int32, device=dev)
@@ -450,9 +451,16 @@ class _DecodeGraph:
             res = m._forward_rows(self.ids, self.pos, self.meta, self.last)
         torch.cuda.current_stream(m.dev).wait_stream(side)
         torch.cuda.synchronize(m.dev)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.out = m._forward_rows(self.ids, self.pos, self.meta, self.last)
+        graph = torch.cuda.CUDAGraph()
+        collecting = gc.isenabled()
+        gc.disable()  # a graph or an event that the collector destroyed meanwhile would invalidate the capture
+        try:
+            with torch.cuda.graph(graph):
+                self.out = m._forward_rows(self.ids, self.pos, self.meta, self.last)
+        finally:
+            if collecting:
+                gc.enable()
+        self.graph = graph
         return res
 
 

@@ -139,3 +139,52 @@ def test_engine_cuda_graph_decode_matches_eager(cuda_device):
         assert [len(o) for o in outs[graphs]] == steps
     assert outs[True] == outs[False]
     assert M.paged.device_error(0) == (0, 0)
+
+
+def test_capture_survives_garbage_that_holds_graphs(cuda_device):
+    """A CUDA graph that Python's collector destroys while another is captured invalidates that capture: the collector
+    rests during one, and a model with its graphs is no cycle that waits for it."""
+    import gc
+    import weakref
+
+    cfg = R.QwenShape(hidden=256, layers=1, hq=14, hkv=2, head_dim=64, inter=512, vocab=1000)
+    w = R.random_weights(cfg, seed=1)
+
+    def engine():
+        model = M.QwenPagedModel(shape_of(cfg), w, 64, 16)
+        sched = host.Scheduler(64, 16, eos_token_ids=(cfg.vocab,))
+        sched.add_request(0, np.arange(5, dtype=np.uint32), max_new_tokens=5)
+        return M.Engine(model, sched), sched
+
+    eng, sched = engine()
+    eng.run()
+    want, old = sched.request_output(0), weakref.ref(eng.model)
+    gc.collect()
+    threshold = gc.get_threshold()
+    gc.disable()
+    try:
+        del eng
+        assert old() is None
+        graph, x = torch.cuda.CUDAGraph(), torch.zeros(8, device="cuda")
+        with torch.cuda.graph(graph):
+            x.add_(1)
+        cycle = [graph]
+        cycle.append(cycle)
+        del graph, cycle
+        eng, sched = engine()
+        rows = eng.model._forward_rows
+
+        def collecting(*a):
+            if torch.cuda.is_current_stream_capturing():
+                gc.set_threshold(1)
+                [[] for _ in range(100)]
+            return rows(*a)
+
+        eng.model._forward_rows = collecting
+        gc.enable()
+        eng.run()
+    finally:
+        gc.set_threshold(*threshold)
+        gc.enable()
+    assert sched.request_output(0) == want
+    gc.collect()
